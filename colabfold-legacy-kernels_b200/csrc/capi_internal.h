@@ -8,8 +8,8 @@ namespace cflk {
 
 // return codes of every entry point (the XLA FFI handler maps them to ffi::Error kinds)
 enum Status : int { kOk = 0, kInvalidArgument = 1, kInternal = 2 };
-// element type of the 16-bit buffers
-enum DType : int { kF16 = 0, kBF16 = 1 };
+// element type of the 16-bit buffers (kF32 only where an entry point says so)
+enum DType : int { kF16 = 0, kBF16 = 1, kF32 = 2 };
 
 constexpr int kMaxDevices = 64;
 
@@ -23,6 +23,7 @@ unsigned read_and_clear_status_bwd();
 unsigned read_and_clear_status_fused();
 unsigned read_and_clear_status_gemm();
 unsigned read_and_clear_status_opm();
+unsigned read_and_clear_status_xent();
 
 // VoltaOpmOuter fused at C = E = 32 (the caller has validated the sizes); the workspace holds
 // wT laid out chunk by chunk (F * 2 KB)

@@ -1,0 +1,1410 @@
+// Softmax cross entropy of a linear layer's classes without keeping the logits, and its gradients.
+//
+//   l = x w^T + b (T tokens, V classes, C channels);  lse = log sum_v exp l;  loss = lse - l[label]
+//   g = dloss (softmax(l) - onehot(label));  dx = g w;  dw = g^T x;  db = sum_t g
+//
+// A token whose label lies outside [0, V) has no loss and no gradient; its row of x is never used
+// (it may hold anything). The labelled rows are gathered into consecutive rows first, so the
+// products cost what the labelled tokens cost; their number stays on the device, where every
+// kernel reads it.
+//
+//   * one persistent GEMM kernel serves the four products: a pair of CTAs (cta_group::2) computes
+//     256 x 256 tiles, each CTA streaming its 128 rows of A and its 128 of B by TMA through a ring
+//     of five 32 KB stages, the leader issuing the MMAs into one of two tensor-memory
+//     accumulators, two warpgroups a CTA draining the other;
+//   * forward: the epilogue reduces each row's 128 columns to (max, sum of exponentials) in the
+//     log2 domain, a second kernel joins a row's pieces in order;
+//   * backward: the classes are taken in pieces; per piece the epilogue turns recomputed logits
+//     into g, rounded to the 16-bit type into the workspace, and g is multiplied by w (adding to
+//     float32 sums of dx) and, transposed, by x. The rounding of g (relative 2^-9 in bf16, 2^-12
+//     in f16) is of the size of the outputs' own rounding and is what feeding the tensor cores
+//     takes; dloss is first scaled by a power of two that brings its largest magnitude to 2^13,
+//     so that f16 keeps g's small values, and the factor is taken out before the outputs round;
+//   * sums, exponentials and row statistics are float32; products whose tiles are too few for the
+//     machine are split along K into float32 slabs added in order. No atomics: the same bits
+//     every run.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <string>
+
+#include "capi_internal.h"
+#include "cflk_b200.h"
+#include "pair_mma.cuh"
+#include "sm100.cuh"
+#include "tmap.h"
+#include "vec_io.cuh"
+
+namespace cflk {
+namespace {
+
+__device__ unsigned g_status;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kInf = __builtin_huge_valf();
+
+// ------------------------------------------------------------------------------------------
+// the labelled tokens
+// ------------------------------------------------------------------------------------------
+constexpr int kPrepThreads = 256, kPrepItems = 1024;  // tokens a block
+
+template <typename L>
+__device__ __forceinline__ int label_of(const L* labels, long long t, long long V) {
+    const long long l = (long long)labels[t];
+    return l >= 0 && l < V ? (int)l : -1;
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    }
+    return x;
+}
+
+__device__ __forceinline__ int warp_sum(int x) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, d);
+    }
+    return x;
+}
+
+// counts[b]: the block's labelled tokens; maxs[b]: the largest finite |dloss| among them (backward)
+template <typename L>
+__global__ void __launch_bounds__(kPrepThreads)
+    xent_count_kernel(const L* __restrict__ labels, const float* __restrict__ dloss, int T,
+                      long long V, int* __restrict__ counts, float* __restrict__ maxs) {
+    __shared__ int sc[8];
+    __shared__ float sm[8];
+    int n = 0;
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < kPrepItems / kPrepThreads; ++j) {
+        const long long t = (long long)blockIdx.x * kPrepItems + j * kPrepThreads + threadIdx.x;
+        if (t < T && label_of(labels, t, V) >= 0) {
+            ++n;
+            if (dloss != nullptr) {
+                const float d = fabsf(dloss[t]);
+                m = d < kInf ? fmaxf(m, d) : m;
+            }
+        }
+    }
+    n = warp_sum(n);
+    m = warp_max(m);
+    if ((threadIdx.x & 31) == 0) {
+        sc[threadIdx.x >> 5] = n;
+        sm[threadIdx.x >> 5] = m;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int s = 0;
+        float mm = 0.f;
+        for (int i = 0; i < 8; ++i) {
+            s += sc[i];
+            mm = fmaxf(mm, sm[i]);
+        }
+        counts[blockIdx.x] = s;
+        maxs[blockIdx.x] = mm;
+    }
+}
+
+// The power of two that brings a positive finite m into [2^13, 2^14); 1 for 0
+__device__ __forceinline__ float grad_scale(float m) {
+    if (!(m > 0.f)) {
+        return 1.f;
+    }
+    int e;
+    frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
+    return exp2f((float)min(14 - e, 126));
+}
+
+struct PrepArgs {
+    const float* dloss;  // backward, with lse
+    const float* lse;
+    float* loss;         // forward: rows without a label get 0 and lse -inf
+    float* lse_out;
+    const int* counts;
+    const float* maxs;
+    int T, nblocks;
+    long long V;
+    int* perm;           // [T]: the labelled tokens in order, the others from the end
+    int* lab;            // labels of the labelled tokens
+    float* lse_c;        // their lse and scaled dloss (backward)
+    float* dl_c;
+    int* count;          // labelled tokens
+    float* inv;          // 1 / grad_scale
+};
+
+// Blocks put their tokens at their places: thread i holds 4 consecutive tokens.
+template <typename L>
+__global__ void __launch_bounds__(kPrepThreads)
+    xent_compact_kernel(const L* __restrict__ labels, const PrepArgs a) {
+    __shared__ int sc[8], so[8];
+    __shared__ float sm[8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // labelled tokens before this block, and the largest |dloss| of all
+    int before = 0;
+    float m = 0.f;
+    for (int i = tid; i < a.nblocks; i += kPrepThreads) {
+        before += i < (int)blockIdx.x ? a.counts[i] : 0;
+        m = fmaxf(m, a.maxs[i]);
+    }
+    before = warp_sum(before);
+    m = warp_max(m);
+    const long long t0 = (long long)blockIdx.x * kPrepItems + tid * 4;
+    int lab[4], mine = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        lab[j] = t0 + j < a.T ? label_of(labels, t0 + j, a.V) : -1;
+        mine += lab[j] >= 0;
+    }
+    int x = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        x += lane >= d ? y : 0;
+    }
+    if (lane == 31) {
+        so[warp] = x;
+    }
+    if (lane == 0) {
+        sc[warp] = before;
+        sm[warp] = m;
+    }
+    __syncthreads();
+    before = 0;
+    int at = x - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        before += sc[w];
+        m = fmaxf(m, sm[w]);
+        at += w < warp ? so[w] : 0;
+        total += so[w];
+    }
+    at += before;
+    const float scale = grad_scale(m);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const long long t = t0 + j;
+        if (t < a.T) {
+            if (lab[j] >= 0) {
+                a.perm[at] = (int)t;
+                a.lab[at] = lab[j];
+                if (a.dloss != nullptr) {
+                    a.lse_c[at] = a.lse[t];
+                    a.dl_c[at] = a.dloss[t] * scale;
+                }
+                ++at;
+            } else {
+                // t - at tokens without a label come before this one
+                a.perm[a.T - 1 - (t - at)] = (int)t;
+                if (a.loss != nullptr) {
+                    a.loss[t] = 0.f;
+                    a.lse_out[t] = -kInf;
+                }
+            }
+        }
+    }
+    if (blockIdx.x == gridDim.x - 1 && tid == 0) {
+        *a.count = before + total;
+        *a.inv = 1.f / scale;
+    }
+}
+
+// xc[i] = x[perm[i]] for the labelled tokens, zeros up to the next multiple of 64 (the K slices
+// of dw read that far); a warp a row, 16 bytes a lane.
+__global__ void __launch_bounds__(256)
+    xent_gather_kernel(const uint4* __restrict__ x, const int* __restrict__ perm,
+                       const int* __restrict__ count, uint4* __restrict__ xc, int cv) {
+    const int n = *count, lane = threadIdx.x & 31;
+    const int end = (n + 63) & ~63;
+    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < end;
+         i += (long long)gridDim.x * 8) {
+        const uint4* src = i < n ? x + (long long)perm[i] * cv : nullptr;
+        uint4* dst = xc + i * cv;
+        for (int c = lane; c < cv; c += 128) {
+            uint4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                v[u] = src != nullptr && c + 32 * u < cv ? src[c + 32 * u] : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (c + 32 * u < cv) {
+                    dst[c + 32 * u] = v[u];
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// the products
+// ------------------------------------------------------------------------------------------
+// kStats: rows of x w^T to (max, sum) pieces; kGrad: to g (16-bit); kDx: g w to float32 slabs;
+// kDw: g^T x to the 16-bit output; kDwSlab: g^T x to float32 slabs.
+enum Kind : int { kStats = 0, kGrad = 1, kDx = 2, kDw = 3, kDwSlab = 4 };
+
+constexpr int PN = 256, PM = 256, PK = 64;  // a pair's tile, and the depth of a stage
+constexpr int kGemmThreads = 384;           // TMA warp, MMA warp, two idle, two epilogue warpgroups
+constexpr int kEpiWarp0 = 4;
+constexpr int kStages = 5;
+constexpr int kHalfBytes = 128 * PK * 2;    // a CTA's rows of A, or of B, in a stage
+constexpr int kStageBytes = 2 * kHalfBytes;
+constexpr int kBoxBytes = 128 * 128;        // output staging: 128 rows of 128 bytes
+constexpr int kSmemBytes = kStages * kStageBytes + 4 * kBoxBytes + 1024;
+static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+constexpr unsigned long long kDrainLimitNs = 200000000ull;
+
+struct GemmArgs {
+    const int* count;     // labelled tokens
+    int row0, rows;       // kStats: the rows of this launch
+    int V, C;
+    int v0, vp;           // the piece of the classes (vp a multiple of 256)
+    int splits;           // along K (kDx, kDwSlab)
+    int accumulate;       // kDx: add to the slab
+    long long cap;        // rows of a statistics piece
+    const int* lab;
+    const void* bias;     // or null
+    float2* part;         // kStats
+    float* lab_logit;     // natural units: a masked label's lowest value stays finite
+    const float* lse_c;   // kGrad
+    const float* dl_c;
+    const float* inv;     // kDw
+};
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::
+                     "l"(map),
+                 "r"(src), "r"(c0), "r"(c1)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1,
+                                             int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::
+            "l"(map),
+        "r"(src), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1,
+                                           int c2) {
+    asm volatile(
+        "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], "
+        "[%1];" ::"l"(map),
+        "r"(src), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
+__device__ __forceinline__ void bulk_commit() {
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() {
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// The output tile and K range of an item; rows fastest, so the pairs at work share B in L2.
+struct Item {
+    int m0, n0, split, kb0, kb1;
+};
+
+template <int KIND>
+struct Schedule {
+    int ntm, ntn, nkb, splits;
+    __device__ __forceinline__ Schedule(const GemmArgs& a, int n) {
+        constexpr bool kDwLike = KIND == kDw || KIND == kDwSlab;
+        const int rows = KIND == kStats ? max(0, min(a.rows, n - a.row0)) : n;
+        const int classes = min(a.vp, a.V - a.v0);
+        ntm = ((kDwLike ? classes : rows) + PM - 1) / PM;
+        ntn = ((KIND == kStats || KIND == kGrad ? classes : a.C) + PN - 1) / PN;
+        const int k = kDwLike ? n : KIND == kDx ? classes : a.C;
+        nkb = (k + PK - 1) / PK;
+        splits = KIND == kDx || KIND == kDwSlab ? a.splits : 1;
+    }
+    __device__ __forceinline__ long long items() const {
+        return (long long)ntm * ntn * splits;
+    }
+    __device__ __forceinline__ Item at(long long i) const {
+        Item r;
+        const int tiles = ntm * ntn;
+        r.split = (int)(i / tiles);
+        const int t = (int)(i - (long long)r.split * tiles);
+        r.n0 = t / ntm * PN;
+        r.m0 = t % ntm * PM;
+        r.kb0 = (int)((long long)nkb * r.split / splits);
+        r.kb1 = (int)((long long)nkb * (r.split + 1) / splits);
+        return r;
+    }
+};
+
+template <typename T, int KIND>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+    xent_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+                     const __grid_constant__ CUtensorMap to, const GemmArgs a) {
+    using E = Elem<T>;
+    constexpr bool A_MN = KIND == kDw || KIND == kDwSlab;
+    constexpr bool B_MN = KIND >= kDx;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+    __shared__ uint32_t tmem_sh;
+    __shared__ int abort_flag;
+    __shared__ __align__(16) float bias_sh[2][128];  // each warpgroup's columns of the tile
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int n = *a.count;
+    const Schedule<KIND> sched(a, n);
+    const long long items = sched.items(), pair0 = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    if (warp == 1) {
+        if (lane == 0) {
+            for (int i = 0; i < kStages; ++i) {
+                mbar_init(&full[i], 1);
+                mbar_init(&empty[i], 1);
+            }
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&acc_full[i], 1);
+                mbar_init(&acc_empty[i], 16);  // eight epilogue warps of each CTA
+            }
+            mbar_init(&drain, 1);
+            abort_flag = 0;
+            fence_mbar_init();
+        }
+        __syncwarp();
+        tmem_alloc_pair(&tmem_sh, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = tmem_sh;
+
+    if (warp == 0 && lane == 0) {
+        // TMA: this CTA's halves of A and B; the leader's barrier counts both CTAs' bytes. A
+        // stage is refilled once the MMAs that read it are done (in both CTAs).
+        int g = 0;
+        bool ok = true;
+        for (long long i = pair0; ok && i < items; i += pairs) {
+            const Item it = sched.at(i);
+            for (int kb = it.kb0; kb < it.kb1; ++kb, ++g) {
+                const int s = g % kStages;
+                if (g >= kStages && !mbar_wait(&empty[s], ((g - kStages) / kStages) & 1, &g_status,
+                                               kStatusMmaWait, &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t* st = smem + s * kStageBytes;
+                uint8_t* sb = st + kHalfBytes;
+                const int k0 = kb * PK;
+                if (rank == 0) {
+                    mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
+                }
+                const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
+                const int m = it.m0 + 128 * (int)rank + (KIND == kStats ? a.row0 : 0);
+                const int nn = it.n0 + 128 * (int)rank;
+                if constexpr (A_MN) {
+                    tma_load_2d_pair(st, &ta, bar, m, k0);
+                    tma_load_2d_pair(st + kHalfBytes / 2, &ta, bar, m + 64, k0);
+                } else {
+                    tma_load_2d_pair(st, &ta, bar, k0, m);
+                }
+                if constexpr (B_MN) {
+                    const int kr = KIND == kDx ? a.v0 + k0 : k0;
+                    tma_load_2d_pair(sb, &tb, bar, nn, kr);
+                    tma_load_2d_pair(sb + kHalfBytes / 2, &tb, bar, nn + 64, kr);
+                } else {
+                    tma_load_2d_pair(sb, &tb, bar, k0, a.v0 + nn);
+                }
+            }
+        }
+        if (rank == 0) {
+            // the last loads (one a stage at most) land before the pair can exit
+            for (int h = g > kStages ? g - kStages : 0; h < g; ++h) {
+                mbar_wait(&full[h % kStages], (h / kStages) & 1, &g_status, kStatusTmaWait,
+                          nullptr, kDrainLimitNs);
+            }
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        const uint32_t idesc = idesc_f16(E::kBf16, PM, PN, A_MN, B_MN);
+        // K-major: rows of 128 bytes (8-row groups 1 KB apart), a K step of 16 is 32 bytes along
+        // the row; MN-major: 64-wide atoms 8 KB apart, a K step is 16 rows of 128 bytes
+        const auto desc = [](uint32_t base, int ks, bool mn) -> uint64_t {
+            return mn ? smem_desc(base + ks * 16 * 128, 64 * 128, 1024, kSwizzle128B)
+                      : smem_desc(base + 32 * ks, 16, 1024, kSwizzle128B);
+        };
+        int g = 0, lt = 0;
+        bool ok = true;
+        for (long long i = pair0; ok && i < items; i += pairs) {
+            const Item it = sched.at(i);
+            if (it.kb0 == it.kb1) {
+                continue;
+            }
+            const int buf = lt & 1;
+            if (lt >= 2 && !mbar_wait(&acc_empty[buf], ((lt - 2) >> 1) & 1, &g_status,
+                                      kStatusSyncWait, &abort_flag)) {
+                break;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * PN;
+            for (int kb = it.kb0; kb < it.kb1; ++kb, ++g) {
+                const int s = g % kStages;
+                if (!mbar_wait(&full[s], (g / kStages) & 1, &g_status, kStatusTmaWait,
+                               &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t sa = smem_u32(smem + s * kStageBytes), sb = sa + kHalfBytes;
+#pragma unroll
+                for (int ks = 0; ks < PK / 16; ++ks) {
+                    mma_ss_pair(acc, desc(sa, ks, A_MN), desc(sb, ks, B_MN), idesc,
+                                kb > it.kb0 || ks > 0 ? 1u : 0u);
+                }
+                mma_commit_pair(&empty[s]);
+            }
+            if (ok) {
+                mma_commit_pair(&acc_full[buf]);
+            }
+            ++lt;
+        }
+        // every MMA issued is complete before tensor memory is freed
+        mma_commit_pair(&drain);
+        mbar_wait(&drain, 0, &g_status, kStatusMmaWait, nullptr, kDrainLimitNs);
+    } else if (warp >= kEpiWarp0) {
+        // epilogue: warpgroup g takes columns [128 g, 128 g + 128) of the CTA's 128 rows (thread r
+        // = row = tensor-memory lane), with its own two staging boxes, named barrier and leader
+        const int g = (warp - kEpiWarp0) >> 2;
+        const int r = ((warp & 3) << 5) | lane;
+        const bool leader = lane == 0 && (warp & 3) == 0;
+        const uint32_t lane_base = tmem_lane_base(warp);
+        uint8_t* slots = smem + kStages * kStageBytes + g * 2 * kBoxBytes;
+        int lt = 0, box = 0;
+        // a box of this warpgroup is free once the store of the box two before it has read it
+        const auto next_slot = [&]() -> uint8_t* {
+            if (leader) {
+                bulk_wait_read<1>();
+            }
+            named_sync(1 + g, 128);
+            return slots + (box++ & 1) * kBoxBytes;
+        };
+        [[maybe_unused]] float out_scale = 1.f;
+        if constexpr (KIND == kDw) {
+            out_scale = *a.inv;
+        }
+        for (long long i = pair0; i < items; i += pairs) {
+            const Item it = sched.at(i);
+            const bool none = it.kb0 == it.kb1;  // an empty K range: zeros
+            const int buf = lt & 1;
+            const int row = it.m0 + 128 * (int)rank + r;  // of the launch's rows
+            const int col0 = it.n0 + 128 * g;
+            [[maybe_unused]] int lab = INT_MIN / 2;  // relative to the piece; no token
+            [[maybe_unused]] float lse2 = 0.f, dl = 0.f;
+            if constexpr (KIND == kStats || KIND == kGrad) {
+                const int tok = row + (KIND == kStats ? a.row0 : 0);
+                if (tok < n) {
+                    lab = a.lab[tok] - a.v0;
+                    if constexpr (KIND == kGrad) {
+                        lse2 = a.lse_c[tok];
+                        dl = a.dl_c[tok];
+                    }
+                }
+                if (a.bias != nullptr) {
+                    named_sync(1 + g, 128);  // the previous tile's reads are done
+                    const int c = a.v0 + col0 + r;
+                    bias_sh[g][r] = c < a.V ? E::to_f(static_cast<const T*>(a.bias)[c]) : 0.f;
+                    named_sync(1 + g, 128);
+                }
+            }
+            if (!none) {
+                mbar_wait(&acc_full[buf], (lt >> 1) & 1, &g_status, kStatusMmaWait, &abort_flag);
+                tc_fence_after();
+                ++lt;
+            }
+            const uint32_t acc = tmem + buf * PN + 128 * g + lane_base;
+            // the accumulator's 32 columns of chunk ch
+            const auto load = [&](int ch, uint32_t (&v)[32]) {
+                tmem_ld32(acc + 32 * ch, v);
+                tmem_wait_ld();
+            };
+            if constexpr (KIND == kStats) {
+                // log2-domain maximum and sum of this row's columns; -inf where nothing is left
+                float m = -kInf, s = 0.f;
+                const int limit = min(a.vp, a.V - a.v0);
+                for (int ch = 0; ch < 4; ++ch) {
+                    const int c0 = col0 + 32 * ch;
+                    if (c0 >= limit) {
+                        break;
+                    }
+                    uint32_t v[32];
+                    load(ch, v);
+                    float y[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        y[j] = __uint_as_float(v[j]);
+                    }
+                    if (a.bias != nullptr) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            y[j] += bias_sh[g][32 * ch + j];
+                        }
+                    }
+                    if (c0 + 32 > limit) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            y[j] = c0 + j < limit ? y[j] : -kInf;
+                        }
+                    }
+                    const int at = lab - c0;
+                    if (at >= 0 && at < 32) {
+                        float z = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            z = j == at ? y[j] : z;
+                        }
+                        a.lab_logit[row + a.row0] = z;
+                    }
+                    float top = y[0];
+#pragma unroll
+                    for (int j = 1; j + 1 < 32; j += 2) {
+                        top = max3(top, y[j], y[j + 1]);
+                    }
+                    top = fmaxf(top, y[31]);
+                    const float m1 = fmaxf(m, top * kLog2e);
+                    const float ref = m1 == -kInf ? 0.f : m1;
+                    float part = 0.f, part1 = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        part += ex2(fmaf(y[j], kLog2e, -ref));
+                        part1 += ex2(fmaf(y[j + 1], kLog2e, -ref));
+                    }
+                    s = s * ex2(m - ref) + (part + part1);
+                    m = m1;
+                }
+                const int piece = (it.n0 / PN) * 2 + g;
+                a.part[piece * a.cap + row] = make_float2(m, s);
+            } else if constexpr (KIND == kGrad) {
+                const int limit = min(a.vp, a.V - a.v0);
+                const bool dead = lse2 == -kInf || lab == INT_MIN / 2;  // nothing left, or no token
+                for (int j = 0; j < 2; ++j) {
+                    const int b0 = col0 + 64 * j;
+                    if (b0 >= limit) {
+                        break;
+                    }
+                    uint8_t* dst = next_slot() + r * 128;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int c0 = b0 + 32 * h;
+                        uint32_t v[32];
+                        load(2 * j + h, v);
+                        float y[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            y[k] = __uint_as_float(v[k]);
+                        }
+                        if (a.bias != nullptr) {
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {
+                                y[k] += bias_sh[g][64 * j + 32 * h + k];
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            y[k] = ex2(fmaf(y[k], kLog2e, -lse2));
+                        }
+                        const int at = lab - c0;
+                        if (at >= 0 && at < 32) {
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {
+                                y[k] -= k == at ? 1.f : 0.f;
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            y[k] = dead || c0 + k >= limit ? 0.f : y[k] * dl;
+                        }
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            *reinterpret_cast<uint4*>(dst + (((4 * h + q) ^ (r & 7)) << 4)) =
+                                make_uint4(E::pack(y[8 * q], y[8 * q + 1]),
+                                           E::pack(y[8 * q + 2], y[8 * q + 3]),
+                                           E::pack(y[8 * q + 4], y[8 * q + 5]),
+                                           E::pack(y[8 * q + 6], y[8 * q + 7]));
+                        }
+                    }
+                    fence_async_smem();
+                    named_sync(1 + g, 128);
+                    if (leader) {
+                        tma_store_2d(&to, smem_u32(dst), b0, it.m0 + 128 * (int)rank);
+                        bulk_commit();
+                    }
+                }
+            } else if constexpr (KIND == kDw) {
+                for (int j = 0; j < 2; ++j) {
+                    const int b0 = col0 + 64 * j;
+                    if (b0 >= a.C) {
+                        break;
+                    }
+                    uint8_t* dst = next_slot() + r * 128;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t v[32];
+                        if (!none) {
+                            load(2 * j + h, v);
+                        }
+                        float y[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            y[k] = none ? 0.f : __uint_as_float(v[k]) * out_scale;
+                        }
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            *reinterpret_cast<uint4*>(dst + (((4 * h + q) ^ (r & 7)) << 4)) =
+                                make_uint4(E::pack(y[8 * q], y[8 * q + 1]),
+                                           E::pack(y[8 * q + 2], y[8 * q + 3]),
+                                           E::pack(y[8 * q + 4], y[8 * q + 5]),
+                                           E::pack(y[8 * q + 6], y[8 * q + 7]));
+                        }
+                    }
+                    fence_async_smem();
+                    named_sync(1 + g, 128);
+                    if (leader) {
+                        const int orow = a.v0 + it.m0 + 128 * (int)rank;
+                        if (orow < a.V) {
+                            tma_store_2d(&to, smem_u32(dst), b0, orow);
+                        }
+                        bulk_commit();
+                    }
+                }
+            } else {
+                for (int ch = 0; ch < 4; ++ch) {
+                    const int c0 = col0 + 32 * ch;
+                    if (c0 >= a.C) {
+                        break;
+                    }
+                    uint32_t v[32];
+                    if (!none) {
+                        load(ch, v);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            v[k] = 0;
+                        }
+                    }
+                    uint8_t* dst = next_slot() + r * 128;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        *reinterpret_cast<uint4*>(dst + ((q ^ (r & 7)) << 4)) =
+                            make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    }
+                    fence_async_smem();
+                    named_sync(1 + g, 128);
+                    if (leader) {
+                        const int orow = it.m0 + 128 * (int)rank;
+                        if (KIND == kDx && a.accumulate) {
+                            tma_add_3d(&to, smem_u32(dst), c0, orow, it.split);
+                        } else {
+                            tma_store_3d(&to, smem_u32(dst), c0, orow, it.split);
+                        }
+                        bulk_commit();
+                    }
+                }
+            }
+            if (!none) {
+                // this warp's columns of the accumulator are read
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive_cluster(map_rank(smem_u32(&acc_empty[buf]), 0));
+                }
+            }
+        }
+        if (leader) {
+            bulk_wait_all();
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (rank == 1 && warp == 1 && lane == 0) {
+        // the leader commits `drain` after every other arrive on this CTA's barriers: once it has
+        // come, none is under way to a CTA that exits
+        mbar_wait(&drain, 0, &g_status, kStatusMmaWait, nullptr, 2 * kDrainLimitNs);
+    }
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while its pair may still signal or load into it
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// joins
+// ------------------------------------------------------------------------------------------
+// Rows' pieces to lse and loss: 32 rows a block, eight threads a row over every eighth piece,
+// joined in order. A row with no class left (every logit -inf) counts as without a label.
+__global__ void __launch_bounds__(256)
+    xent_join_kernel(const float2* __restrict__ part, const float* __restrict__ lab_logit,
+                     const int* __restrict__ perm, const int* __restrict__ count, int row0,
+                     int rows, long long cap, int pieces, float* __restrict__ loss,
+                     float* __restrict__ lse) {
+    __shared__ float2 sh[8][32];
+    const int n = *count;
+    const int r = threadIdx.x & 31, seg = threadIdx.x >> 5;
+    const int row = blockIdx.x * 32 + r;
+    const bool live = row < rows && row0 + row < n;
+    float m = -kInf, s = 0.f;
+    const auto join = [&](float2 p) {
+        const float m1 = fmaxf(m, p.x);
+        const float ref = m1 == -kInf ? 0.f : m1;
+        s = s * ex2(m - ref) + p.y * ex2(p.x - ref);
+        m = m1;
+    };
+    if (live) {
+        for (int p = seg; p < pieces; p += 32) {
+            float2 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                v[u] = p + 8 * u < pieces ? part[(p + 8 * u) * cap + row] : make_float2(-kInf, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                join(v[u]);
+            }
+        }
+    }
+    sh[seg][r] = make_float2(m, s);
+    __syncthreads();
+    if (seg == 0 && live) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+            join(sh[i][r]);
+        }
+        const int t = perm[row0 + row];
+        const bool none = m == -kInf && s == 0.f;
+        const float l2 = log2f(s);
+        lse[t] = none ? -kInf : m + l2;
+        loss[t] = none ? 0.f : kLn2 * (m + l2) - lab_logit[row0 + row];
+    }
+}
+
+// dx rows: the slabs of a labelled token's row added in order, scaled and rounded; zeros for the
+// others. A warp a row, eight channels a lane.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    xent_dx_kernel(const float* __restrict__ acc, long long slab, int splits,
+                   const int* __restrict__ perm, const int* __restrict__ count,
+                   const float* __restrict__ inv, T* __restrict__ dx, int rows, int C) {
+    const int n = *count, lane = threadIdx.x & 31;
+    const float by = *inv;
+    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows;
+         i += (long long)gridDim.x * 8) {
+        T* dst = dx + (long long)perm[i] * C;
+        for (int c = lane * 8; c < C; c += 256) {
+            float s[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                s[k] = 0.f;
+            }
+            if (i < n) {
+                load_vec<float, 8>(acc + i * C + c, s);
+                for (int p = 1; p < splits; ++p) {
+                    float v[8];
+                    load_vec<float, 8>(acc + p * slab + i * C + c, v);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        s[k] += v[k];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    s[k] *= by;
+                }
+            }
+            store_vec<T, 8>(dst + c, s);
+        }
+    }
+}
+
+// dw of a piece from its slabs, eight channels a thread
+template <typename T>
+__global__ void __launch_bounds__(256)
+    xent_dw_kernel(const float* __restrict__ acc, long long slab, int splits,
+                   const float* __restrict__ inv, T* __restrict__ dw, long long total8) {
+    const float by = *inv;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total8;
+         i += (long long)gridDim.x * 256) {
+        float s[8];
+        load_vec<float, 8>(acc + i * 8, s);
+        for (int p = 1; p < splits; ++p) {
+            float v[8];
+            load_vec<float, 8>(acc + p * slab + i * 8, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                s[k] += v[k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            s[k] *= by;
+        }
+        store_vec<T, 8>(dw + i * 8, s);
+    }
+}
+
+constexpr int kBiasChunks = 32;
+
+// column sums of a piece of g: a block 256 columns of one of kBiasChunks row ranges
+template <typename T>
+__global__ void __launch_bounds__(256)
+    xent_colsum_kernel(const T* __restrict__ g, const int* __restrict__ count, int vp, int limit,
+                       float* __restrict__ part) {
+    __shared__ float sh[8][256];
+    const int n = *count;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int col = blockIdx.x * 256 + lane * 8;
+    const int r0 = (int)((long long)n * blockIdx.y / kBiasChunks);
+    const int r1 = (int)((long long)n * (blockIdx.y + 1) / kBiasChunks);
+    float s[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        s[k] = 0.f;
+    }
+    if (col < limit) {  // g holds whole 64-column boxes up to the limit
+        for (int r = r0 + w; r < r1; r += 32) {
+            float v[4][8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (r + 8 * u < r1) {
+                    load_vec<T, 8>(g + (long long)(r + 8 * u) * vp + col, v[u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (r + 8 * u < r1) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        s[k] += v[u][k];
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        sh[w][lane * 8 + k] = s[k];
+    }
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        t += sh[i][threadIdx.x];
+    }
+    part[(long long)blockIdx.y * vp + blockIdx.x * 256 + threadIdx.x] = t;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    xent_dbias_kernel(const float* __restrict__ part, int vp, int limit,
+                      const float* __restrict__ inv, T* __restrict__ dbias) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < limit) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < kBiasChunks; ++i) {
+            s += part[(long long)i * vp + c];
+        }
+        dbias[c] = Elem<T>::from_f(s * *inv);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// plans
+// ------------------------------------------------------------------------------------------
+size_t round256(size_t n) {
+    return (n + 255) & ~size_t(255);
+}
+
+constexpr int64_t kMax = int64_t(1) << 31;
+constexpr size_t kPartBytes = size_t(256) << 20;   // statistics pieces of one launch
+constexpr size_t kPieceBytes = size_t(512) << 20;  // g of one piece of the classes
+constexpr int kPairs = 74;
+
+struct Plan {
+    int64_t tp;        // rows of the gathered tokens, whole tiles
+    int64_t row_step;  // forward: rows a launch
+    int64_t vp;        // classes a piece (backward), whole tiles
+    int dx_splits, dw_splits;
+    size_t counts, maxs, perm, lab, lse_c, dl_c, scalars, xc;
+    size_t part, lab_logit;             // forward
+    size_t g, dx_acc, dw_acc, db_part;  // backward
+    size_t bytes;
+};
+
+// False where a size overflows what the kernels index.
+bool make_plan(int64_t T, int64_t V, int64_t C, bool bwd, Plan& p) {
+    if (T >= kMax - 1024 || V >= kMax - 1024 || C >= kMax - 1024) {
+        return false;
+    }
+    int64_t mul = 0;
+    if (__builtin_mul_overflow(T + 256, C * 64, &mul) || __builtin_mul_overflow(V, C * 64, &mul)) {
+        return false;
+    }
+    p.tp = (T + PM - 1) / PM * PM;
+    const int64_t tiles_v = (V + PN - 1) / PN, tiles_c = (C + PN - 1) / PN, tiles_t = p.tp / PM;
+    size_t at = 0;
+    const auto take = [&](size_t n) {
+        const size_t o = at;
+        at += round256(n);
+        return o;
+    };
+    const int64_t nb = (T + kPrepItems - 1) / kPrepItems;
+    p.counts = take(nb * 4);
+    p.maxs = take(nb * 4);
+    p.perm = take(T * 4);
+    p.lab = take(T * 4);
+    p.scalars = take(256);
+    p.xc = take((size_t)p.tp * C * 2);
+    if (!bwd) {
+        const int64_t row_bytes = tiles_v * 2 * 8;
+        p.row_step = std::min<int64_t>(
+            p.tp, std::max<int64_t>(PM, (int64_t)kPartBytes / row_bytes / PM * PM));
+        p.part = take((size_t)p.row_step * row_bytes);
+        p.lab_logit = take(p.tp * 4);
+    } else {
+        p.lse_c = take(T * 4);
+        p.dl_c = take(T * 4);
+        // pieces of equal size, whole tiles, each at most kPieceBytes of g
+        const int64_t most = std::max<int64_t>(1, (int64_t)kPieceBytes / (p.tp * 2) / PN);
+        const int64_t pieces = (tiles_v + most - 1) / most;
+        p.vp = (tiles_v + pieces - 1) / pieces * PN;
+        const int64_t tiles_p = p.vp / PN;
+        // K is split where the tiles leave pairs idle, into ranges of at least 8 stages
+        const auto splits = [](int64_t tiles, int64_t k) {
+            const int64_t most_k = std::max<int64_t>(1, k / (8 * PK));
+            return (int)std::max<int64_t>(1, std::min<int64_t>(most_k, kPairs / tiles));
+        };
+        p.dx_splits = splits(tiles_t * tiles_c, p.vp);
+        p.dw_splits = splits(tiles_p * tiles_c, T);
+        p.g = take((size_t)p.tp * p.vp * 2);
+        p.dx_acc = take((size_t)p.dx_splits * p.tp * C * 4);
+        p.dw_acc = p.dw_splits > 1 ? take((size_t)p.dw_splits * p.vp * C * 4) : 0;
+        p.db_part = take((size_t)kBiasChunks * p.vp * 4);
+    }
+    p.bytes = at;
+    return true;
+}
+
+template <typename T, int KIND>
+cudaError_t launch_gemm(cudaStream_t s, const CUtensorMap& ta, const CUtensorMap& tb,
+                        const CUtensorMap& to, const GemmArgs& a, int64_t items) {
+    auto kern = xent_gemm_kernel<T, KIND>;
+    // the pairs that fit the device at once, found once a device
+    static int pairs[kMaxDevices] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    if (dev >= kMaxDevices || pairs[dev] == 0) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * kPairs);
+        cfg.blockDim = dim3(kGemmThreads);
+        cfg.dynamicSmemBytes = kSmemBytes;
+        int fit = 0;
+        e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        fit = std::max(1, std::min(fit, kPairs));
+        if (dev >= kMaxDevices) {
+            kern<<<2 * (unsigned)std::min<int64_t>(items, fit), kGemmThreads, kSmemBytes, s>>>(
+                ta, tb, to, a);
+            return cudaGetLastError();
+        }
+        pairs[dev] = fit;
+    }
+    const unsigned grid = 2 * (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, pairs[dev]));
+    kern<<<grid, kGemmThreads, kSmemBytes, s>>>(ta, tb, to, a);
+    return cudaGetLastError();
+}
+
+// a row-major [rows][cols] matrix in boxes of box_cols x box_rows (128-byte rows)
+bool map2(CUtensorMap* m, CUtensorMapDataType t, int es, const void* p, int64_t rows, int64_t cols,
+          uint32_t box_rows) {
+    const uint64_t d[2] = {(uint64_t)cols, (uint64_t)rows}, st[1] = {(uint64_t)cols};
+    const uint32_t box[2] = {(uint32_t)(128 / es), box_rows};
+    return encode_tiled(m, t, es, 2, p, d, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+bool map3(CUtensorMap* m, const void* p, int64_t slabs, int64_t rows, int64_t cols) {
+    const uint64_t d[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)slabs};
+    const uint64_t st[2] = {(uint64_t)cols, (uint64_t)(cols * rows)};
+    const uint32_t box[3] = {32, 128, 1};
+    return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, 3, p, d, st, box,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+struct Call {
+    cudaStream_t s;
+    int dtype, labels_64;
+    const void *x, *w, *bias, *labels;
+    const float *lse_in, *dloss;
+    float *loss, *lse;
+    void *dx, *dw, *dbias;
+    int64_t T, V, C;
+    uint8_t* ws;
+};
+
+// label compaction and the gather of x
+cudaError_t prepare(const Call& c, const Plan& p) {
+    const int64_t nb = (c.T + kPrepItems - 1) / kPrepItems;
+    PrepArgs a{};
+    a.dloss = c.dloss;
+    a.lse = c.lse_in;
+    a.loss = c.loss;
+    a.lse_out = c.lse;
+    a.counts = reinterpret_cast<int*>(c.ws + p.counts);
+    a.maxs = reinterpret_cast<float*>(c.ws + p.maxs);
+    a.T = (int)c.T;
+    a.nblocks = (int)nb;
+    a.V = c.V;
+    a.perm = reinterpret_cast<int*>(c.ws + p.perm);
+    a.lab = reinterpret_cast<int*>(c.ws + p.lab);
+    a.lse_c = reinterpret_cast<float*>(c.ws + p.lse_c);
+    a.dl_c = reinterpret_cast<float*>(c.ws + p.dl_c);
+    a.count = reinterpret_cast<int*>(c.ws + p.scalars);
+    a.inv = reinterpret_cast<float*>(c.ws + p.scalars + 4);
+    int* counts = reinterpret_cast<int*>(c.ws + p.counts);
+    float* maxs = reinterpret_cast<float*>(c.ws + p.maxs);
+    const auto run = [&](auto tag) {
+        using L = decltype(tag);
+        const L* labels = static_cast<const L*>(c.labels);
+        xent_count_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.s>>>(labels, c.dloss, (int)c.T,
+                                                                     c.V, counts, maxs);
+        xent_compact_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.s>>>(labels, a);
+    };
+    if (c.labels_64) {
+        run((long long)0);
+    } else {
+        run(0);
+    }
+    const unsigned grid = (unsigned)std::min<int64_t>((c.T + 63 + 7) / 8, 148 * 8);
+    xent_gather_kernel<<<grid, 256, 0, c.s>>>(static_cast<const uint4*>(c.x), a.perm, a.count,
+                                              reinterpret_cast<uint4*>(c.ws + p.xc),
+                                              (int)(c.C / 8));
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t forward(const Call& c, const Plan& p, bool& map_ok) {
+    const CUtensorMapDataType t =
+        c.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap tx, tw;
+    map_ok = map2(&tx, t, 2, c.ws + p.xc, p.tp, c.C, 128) && map2(&tw, t, 2, c.w, c.V, c.C, 128);
+    if (!map_ok) {
+        return cudaSuccess;
+    }
+    cudaError_t e = prepare(c, p);
+    GemmArgs a{};
+    a.count = reinterpret_cast<int*>(c.ws + p.scalars);
+    a.V = (int)c.V;
+    a.C = (int)c.C;
+    a.vp = (int)((c.V + PN - 1) / PN * PN);
+    a.splits = 1;
+    a.cap = p.row_step;
+    a.lab = reinterpret_cast<int*>(c.ws + p.lab);
+    a.bias = c.bias;
+    a.part = reinterpret_cast<float2*>(c.ws + p.part);
+    a.lab_logit = reinterpret_cast<float*>(c.ws + p.lab_logit);
+    for (int64_t r0 = 0; e == cudaSuccess && r0 < c.T; r0 += p.row_step) {
+        a.row0 = (int)r0;
+        a.rows = (int)std::min(p.row_step, c.T - r0);
+        const int64_t items = (int64_t)((a.rows + PM - 1) / PM) * (a.vp / PN);
+        e = launch_gemm<T, kStats>(c.s, tx, tw, tw, a, items);
+        if (e == cudaSuccess) {
+            xent_join_kernel<<<(a.rows + 31) / 32, 256, 0, c.s>>>(
+                a.part, a.lab_logit, reinterpret_cast<int*>(c.ws + p.perm), a.count, a.row0, a.rows,
+                a.cap, 2 * (a.vp / PN), c.loss, c.lse);
+            e = cudaGetLastError();
+        }
+    }
+    return e;
+}
+
+template <typename T>
+cudaError_t backward(const Call& c, const Plan& p, bool& map_ok) {
+    const CUtensorMapDataType t =
+        c.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    T* g = reinterpret_cast<T*>(c.ws + p.g);
+    float* dx_acc = reinterpret_cast<float*>(c.ws + p.dx_acc);
+    float* dw_acc = reinterpret_cast<float*>(c.ws + p.dw_acc);
+    float* db_part = reinterpret_cast<float*>(c.ws + p.db_part);
+    const float* inv = reinterpret_cast<float*>(c.ws + p.scalars + 4);
+    // K-major operands in boxes of 128 rows, MN-major ones in boxes of 64 K rows
+    CUtensorMap x_k, w_k, g_k, x_n, w_n, g_m, g_out, dx_out, dw_out;
+    map_ok = map2(&x_k, t, 2, c.ws + p.xc, p.tp, c.C, 128) &&
+             map2(&w_k, t, 2, c.w, c.V, c.C, 128) && map2(&g_k, t, 2, g, p.tp, p.vp, 128) &&
+             map2(&x_n, t, 2, c.ws + p.xc, p.tp, c.C, 64) && map2(&w_n, t, 2, c.w, c.V, c.C, 64) &&
+             map2(&g_m, t, 2, g, p.tp, p.vp, 64) && map3(&dx_out, dx_acc, p.dx_splits, p.tp, c.C) &&
+             (p.dw_splits > 1 ? map3(&dw_out, dw_acc, p.dw_splits, p.vp, c.C)
+                              : map2(&dw_out, t, 2, c.dw, c.V, c.C, 128));
+    if (!map_ok) {
+        return cudaSuccess;
+    }
+    g_out = g_k;
+    cudaError_t e = prepare(c, p);
+    GemmArgs a{};
+    a.count = reinterpret_cast<int*>(c.ws + p.scalars);
+    a.V = (int)c.V;
+    a.C = (int)c.C;
+    a.vp = (int)p.vp;
+    a.lab = reinterpret_cast<int*>(c.ws + p.lab);
+    a.bias = c.bias;
+    a.lse_c = reinterpret_cast<float*>(c.ws + p.lse_c);
+    a.dl_c = reinterpret_cast<float*>(c.ws + p.dl_c);
+    a.inv = inv;
+    const int64_t tiles_t = p.tp / PM, tiles_c = (c.C + PN - 1) / PN;
+    for (int64_t v0 = 0; e == cudaSuccess && v0 < c.V; v0 += p.vp) {
+        a.v0 = (int)v0;
+        const int64_t classes = std::min(p.vp, c.V - v0);
+        const int64_t tiles_p = (classes + PN - 1) / PN;
+        a.splits = 1;
+        e = launch_gemm<T, kGrad>(c.s, x_k, w_k, g_out, a, tiles_t * tiles_p);
+        if (e == cudaSuccess && c.dbias != nullptr) {
+            xent_colsum_kernel<T><<<dim3((unsigned)tiles_p, kBiasChunks), 256, 0, c.s>>>(
+                g, a.count, a.vp, (int)classes, db_part);
+            xent_dbias_kernel<T><<<(unsigned)tiles_p, 256, 0, c.s>>>(
+                db_part, a.vp, (int)classes, inv, static_cast<T*>(c.dbias) + v0);
+            e = cudaGetLastError();
+        }
+        if (e == cudaSuccess) {
+            a.splits = p.dx_splits;
+            a.accumulate = v0 > 0;
+            e = launch_gemm<T, kDx>(c.s, g_k, w_n, dx_out, a, tiles_t * tiles_c * a.splits);
+        }
+        if (e == cudaSuccess) {
+            a.splits = p.dw_splits;
+            const int64_t items = tiles_p * tiles_c * a.splits;
+            if (p.dw_splits == 1) {
+                e = launch_gemm<T, kDw>(c.s, g_m, x_n, dw_out, a, items);
+            } else {
+                e = launch_gemm<T, kDwSlab>(c.s, g_m, x_n, dw_out, a, items);
+                if (e == cudaSuccess) {
+                    const int64_t total8 = classes * c.C / 8;
+                    xent_dw_kernel<T><<<(unsigned)std::min<int64_t>((total8 + 255) / 256, 148 * 8),
+                                        256, 0, c.s>>>(dw_acc, p.vp * c.C, a.splits, inv,
+                                                       static_cast<T*>(c.dw) + v0 * c.C, total8);
+                    e = cudaGetLastError();
+                }
+            }
+        }
+    }
+    if (e == cudaSuccess) {
+        xent_dx_kernel<T><<<(unsigned)std::min<int64_t>((c.T + 7) / 8, 148 * 8), 256, 0, c.s>>>(
+            dx_acc, p.tp * c.C, p.dx_splits, reinterpret_cast<int*>(c.ws + p.perm), a.count, inv,
+            static_cast<T*>(c.dx), (int)c.T, (int)c.C);
+        e = cudaGetLastError();
+    }
+    return e;
+}
+
+int check(const char* who, int dtype, int labels_64, int64_t T, int64_t V, int64_t C) {
+    const auto bad = [&](const char* what) {
+        return fail(kInvalidArgument, std::string(who) + ": " + what);
+    };
+    if (dtype != kF16 && dtype != kBF16) {
+        return bad("dtype must be f16 or bf16");
+    }
+    if (labels_64 != 0 && labels_64 != 1) {
+        return bad("labels are int32 (labels_64 0) or int64 (1)");
+    }
+    if (T < 0 || V < 1 || C < 8 || C % 8 != 0) {
+        return bad("T non-negative, V at least 1, C a positive multiple of 8");
+    }
+    return kOk;
+}
+
+int workspace_size(const char* who, int64_t T, int64_t V, int64_t C, bool bwd, size_t* bytes) {
+    const int rc = check(who, kBF16, 0, T, V, C);
+    if (rc != kOk) {
+        return rc;
+    }
+    if (bytes == nullptr) {
+        return fail(kInvalidArgument, std::string(who) + ": null size");
+    }
+    *bytes = 0;
+    Plan p{};
+    if (T > 0) {
+        if (!make_plan(T, V, C, bwd, p)) {
+            return fail(kInvalidArgument, std::string(who) + ": sizes must be below 2^31");
+        }
+        *bytes = p.bytes;
+    }
+    return kOk;
+}
+
+int finish(const char* who, bool map_ok, cudaError_t e) {
+    if (!map_ok) {
+        return fail(kInvalidArgument, std::string(who) + ": TMA descriptor rejected");
+    }
+    if (e != cudaSuccess) {
+        return fail(kInternal, std::string(who) + " launch: " + cudaGetErrorString(e));
+    }
+    return kOk;
+}
+
+int check_workspace(const char* who, const void* ws, size_t have, size_t need) {
+    if (ws == nullptr || have < need || reinterpret_cast<uintptr_t>(ws) % 256 != 0) {
+        return fail(kInvalidArgument,
+                    std::string(who) + ": workspace below the size function's or not 256-byte "
+                                       "aligned");
+    }
+    return kOk;
+}
+
+}  // namespace
+
+unsigned read_and_clear_status_xent() {
+    unsigned v = 0, z = 0;
+    cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
+    cudaMemcpyToSymbol(g_status, &z, sizeof(z));
+    return v;
+}
+
+}  // namespace cflk
+
+using namespace cflk;
+
+extern "C" int cflk_linear_xent_workspace_size(int64_t T, int64_t V, int64_t C, size_t* bytes) {
+    clear_error();
+    return workspace_size("linear_xent", T, V, C, false, bytes);
+}
+
+extern "C" int cflk_linear_xent(void* stream, int dtype, int labels_64, const void* x,
+                                const void* w, const void* bias, const void* labels, float* loss,
+                                float* lse, int64_t T, int64_t V, int64_t C, void* workspace,
+                                size_t ws_bytes) {
+    clear_error();
+    const char* who = "linear_xent";
+    int rc = check(who, dtype, labels_64, T, V, C);
+    if (rc != kOk || T == 0) {
+        return rc;
+    }
+    if (x == nullptr || w == nullptr || labels == nullptr || loss == nullptr || lse == nullptr) {
+        return fail(kInvalidArgument, "linear_xent: null buffer");
+    }
+    if (!aligned16(x) || !aligned16(w)) {
+        return fail(kInvalidArgument, "linear_xent: x and w must be 16-byte aligned");
+    }
+    Plan p{};
+    if (!make_plan(T, V, C, false, p)) {
+        return fail(kInvalidArgument, "linear_xent: sizes must be below 2^31");
+    }
+    rc = check_workspace(who, workspace, ws_bytes, p.bytes);
+    if (rc != kOk) {
+        return rc;
+    }
+    Call c{};
+    c.s = static_cast<cudaStream_t>(stream);
+    c.dtype = dtype;
+    c.labels_64 = labels_64;
+    c.x = x;
+    c.w = w;
+    c.bias = bias;
+    c.labels = labels;
+    c.loss = loss;
+    c.lse = lse;
+    c.T = T;
+    c.V = V;
+    c.C = C;
+    c.ws = static_cast<uint8_t*>(workspace);
+    bool map_ok = true;
+    const cudaError_t e =
+        dtype == kBF16 ? forward<__nv_bfloat16>(c, p, map_ok) : forward<__half>(c, p, map_ok);
+    return finish(who, map_ok, e);
+}
+
+extern "C" int cflk_linear_xent_bwd_workspace_size(int64_t T, int64_t V, int64_t C,
+                                                   size_t* bytes) {
+    clear_error();
+    return workspace_size("linear_xent_bwd", T, V, C, true, bytes);
+}
+
+extern "C" int cflk_linear_xent_bwd(void* stream, int dtype, int labels_64, const void* x,
+                                    const void* w, const void* bias, const void* labels,
+                                    const float* lse, const float* dloss, void* dx, void* dw,
+                                    void* dbias, int64_t T, int64_t V, int64_t C, void* workspace,
+                                    size_t ws_bytes) {
+    clear_error();
+    const char* who = "linear_xent_bwd";
+    int rc = check(who, dtype, labels_64, T, V, C);
+    if (rc != kOk) {
+        return rc;
+    }
+    if (dw == nullptr || (bias == nullptr) != (dbias == nullptr)) {
+        return fail(kInvalidArgument, "linear_xent_bwd: null buffer (dbias goes with bias)");
+    }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (T == 0) {
+        cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)V * (size_t)C * 2, s);
+        if (e == cudaSuccess && dbias != nullptr) {
+            e = cudaMemsetAsync(dbias, 0, (size_t)V * 2, s);
+        }
+        return finish(who, true, e);
+    }
+    if (x == nullptr || w == nullptr || labels == nullptr || lse == nullptr || dloss == nullptr ||
+        dx == nullptr) {
+        return fail(kInvalidArgument, "linear_xent_bwd: null buffer");
+    }
+    if (!aligned16(x) || !aligned16(w) || !aligned16(dx) || !aligned16(dw)) {
+        return fail(kInvalidArgument,
+                    "linear_xent_bwd: x, w, dx and dw must be 16-byte aligned");
+    }
+    Plan p{};
+    if (!make_plan(T, V, C, true, p)) {
+        return fail(kInvalidArgument, "linear_xent_bwd: sizes must be below 2^31");
+    }
+    rc = check_workspace(who, workspace, ws_bytes, p.bytes);
+    if (rc != kOk) {
+        return rc;
+    }
+    Call c{};
+    c.s = s;
+    c.dtype = dtype;
+    c.labels_64 = labels_64;
+    c.x = x;
+    c.w = w;
+    c.bias = bias;
+    c.labels = labels;
+    c.lse_in = lse;
+    c.dloss = dloss;
+    c.dx = dx;
+    c.dw = dw;
+    c.dbias = dbias;
+    c.T = T;
+    c.V = V;
+    c.C = C;
+    c.ws = static_cast<uint8_t*>(workspace);
+    bool map_ok = true;
+    const cudaError_t e =
+        dtype == kBF16 ? backward<__nv_bfloat16>(c, p, map_ok) : backward<__half>(c, p, map_ok);
+    return finish(who, map_ok, e);
+}

@@ -51,6 +51,17 @@ _SIGS = {
     'cflk_volta_opm_outer_workspace_size': [_i64, _i64, _i64, _i64, _C.POINTER(_C.c_size_t)],
     'cflk_volta_opm_outer': [_p, _int, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p,
                              _C.c_size_t],
+    'cflk_embed': [_p, _int, _int, _int, _p, _p, _p, _i64, _i64, _i64, _f32],
+    'cflk_embed_bwd_workspace_size': [_i64, _i64, _i64, _C.POINTER(_C.c_size_t)],
+    'cflk_embed_bwd': [_p, _int, _int, _p, _p, _p, _i64, _i64, _i64, _f32, _p, _C.c_size_t],
+    'cflk_linear_xent_workspace_size': [_i64, _i64, _i64, _C.POINTER(_C.c_size_t)],
+    'cflk_linear_xent': [_p, _int, _int, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p,
+                         _C.c_size_t],
+    'cflk_linear_xent_bwd_workspace_size': [_i64, _i64, _i64, _C.POINTER(_C.c_size_t)],
+    'cflk_linear_xent_bwd': [_p, _int, _int] + [_p] * 9 + [_i64, _i64, _i64, _p, _C.c_size_t],
+    'cflk_grad_workspace_size': [_i64, _C.POINTER(_C.c_size_t)],
+    'cflk_grad_sumsq': [_p, _i64, _p, _p, _p, _p, _p, _C.c_size_t],
+    'cflk_grad_clip': [_p, _i64, _p, _p, _p, _p, _p, _p, _f32, _f32, _f32, _p, _p, _C.c_size_t],
 }
 
 _lib = None
@@ -535,3 +546,160 @@ def volta_transition(x, scale, offset, w1T, b1, w2T, b2, keep, *, eps, add_input
                                      float(eps), int(bool(add_input)))
     _check(rc, who)
     return out
+
+
+# ---- token training -------------------------------------------------------------------------
+
+_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _index_64(t, name, who):
+    if t.dtype == torch.int32:
+        return 0
+    if t.dtype == torch.int64:
+        return 1
+    raise ValueError('%s: %s must be int32 or int64, got %s' % (who, name, t.dtype))
+
+
+def _code(t, name, who):
+    if t.dtype not in _CODES:
+        raise ValueError('%s: %s must be float16, bfloat16 or float32, got %s' %
+                         (who, name, t.dtype))
+    return _CODES[t.dtype]
+
+
+def _workspace(size_fn, args, like, who):
+    n = _C.c_size_t(0)
+    _check(getattr(lib(), size_fn)(*args, _C.byref(n)), who)
+    return torch.empty(max(n.value, 1), dtype=torch.uint8, device=like.device), n.value
+
+
+def embed(ids, table, *, scale=1.0, out_dtype=None, out=None):
+    """Embedding lookup with scaling: out [*ids.shape, C] = scale * table[ids], zeros for an id
+    outside [0, V). ids int32 or int64 of any shape; table [V,C] float16, bfloat16 or float32;
+    out_dtype defaults to the table's type (a float32 table may give any of the three)."""
+    who = 'embed'
+    if table.dim() != 2:
+        raise ValueError('embed: table must be [V,C]')
+    V, C = table.shape
+    i64 = _index_64(ids, 'ids', who)
+    if out is None:
+        out = torch.empty((*ids.shape, C), dtype=out_dtype or table.dtype, device=table.device)
+    if out.numel() != ids.numel() * C or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError('embed: out must be [*ids.shape, C] of out_dtype')
+    rc = lib().cflk_embed(_stream(), _code(table, 'table', who), _code(out, 'out', who), i64,
+                          _ptr(ids), _ptr(table), _ptr(out), ids.numel(), V, C, float(scale))
+    _check(rc, who)
+    return out
+
+
+def embed_bwd(ids, dout, num_rows, *, scale=1.0):
+    """The gradient of embed's table: dtable [num_rows, C] float32, the scaled sum of dout
+    [*ids.shape, C] over the tokens of each row, in a fixed order."""
+    who = 'embed_bwd'
+    if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:
+        raise ValueError('embed_bwd: dout must be [*ids.shape, C]')
+    T, V, C = ids.numel(), int(num_rows), dout.shape[-1]
+    i64, dt = _index_64(ids, 'ids', who), _code(dout, 'dout', who)
+    ws, n = _workspace('cflk_embed_bwd_workspace_size', (T, V, C), dout, who)
+    dtable = torch.empty((V, C), dtype=torch.float32, device=dout.device)
+    rc = lib().cflk_embed_bwd(_stream(), dt, i64, _ptr(ids), _ptr(dout), _ptr(dtable), T, V, C,
+                              float(scale), _ptr(ws), n)
+    _check(rc, who)
+    return dtable
+
+
+def _xent_sizes(x, w, labels, bias, who):
+    if x.dim() < 2 or w.dim() != 2 or w.shape[1] != x.shape[-1] or labels.shape != x.shape[:-1]:
+        raise ValueError('%s: x must be [...,C], w [V,C], labels x.shape[:-1]' % who)
+    if bias is not None and bias.shape != (w.shape[0],):
+        raise ValueError('%s: bias must be [V]' % who)
+    dt = _dtype_code(x, w, *(() if bias is None else (bias,)))
+    return dt, _index_64(labels, 'labels', who), labels.numel(), w.shape[0], x.shape[-1]
+
+
+def linear_xent(x, w, labels, bias=None):
+    """Softmax cross entropy of the classes x w^T + bias without keeping them: (loss, lse), both
+    float32 of labels' shape, lse in the log2 domain. x [...,C], w [V,C], labels int32 or int64
+    [...]; a label outside [0, V) gives loss 0 and lse -inf."""
+    who = 'linear_xent'
+    dt, l64, T, V, C = _xent_sizes(x, w, labels, bias, who)
+    ws, n = _workspace('cflk_linear_xent_workspace_size', (T, V, C), x, who)
+    loss = torch.empty(labels.shape, dtype=torch.float32, device=x.device)
+    lse = torch.empty_like(loss)
+    rc = lib().cflk_linear_xent(_stream(), dt, l64, _ptr(x), _ptr(w), _ptr(bias), _ptr(labels),
+                                _ptr(loss), _ptr(lse), T, V, C, _ptr(ws), n)
+    _check(rc, who)
+    return loss, lse
+
+
+def linear_xent_bwd(x, w, labels, lse, dloss, bias=None):
+    """Gradients of linear_xent for dloss (float32, labels' shape): (dx, dw, dbias), in the types
+    of x, w and bias; dbias is None without a bias."""
+    who = 'linear_xent_bwd'
+    dt, l64, T, V, C = _xent_sizes(x, w, labels, bias, who)
+    if lse.shape != labels.shape or dloss.shape != labels.shape:
+        raise ValueError('linear_xent_bwd: lse and dloss must have the shape of labels')
+    ws, n = _workspace('cflk_linear_xent_bwd_workspace_size', (T, V, C), x, who)
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    dbias = None if bias is None else torch.empty_like(bias)
+    rc = lib().cflk_linear_xent_bwd(_stream(), dt, l64, _ptr(x), _ptr(w), _ptr(bias),
+                                    _ptr(labels), _f32_ptr(lse, 'lse', who),
+                                    _f32_ptr(dloss, 'dloss', who), _ptr(dx), _ptr(dw),
+                                    _ptr(dbias), T, V, C, _ptr(ws), n)
+    _check(rc, who)
+    return dx, dw, dbias
+
+
+def _tensor_table(tensors, who):
+    """(pointers, element counts, type codes) of contiguous CUDA tensors as C arrays."""
+    n = len(tensors)
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise ValueError('%s: tensors must be contiguous' % who)
+    try:
+        codes = [_CODES[t.dtype] for t in tensors]
+    except KeyError as e:
+        raise ValueError('%s: gradients must be float16, bfloat16 or float32, got %s' %
+                         (who, e)) from None
+    if len({t.device for t in tensors}) > 1 or (n and not tensors[0].is_cuda):
+        raise ValueError('%s: tensors must be on one CUDA device' % who)
+    return ((_p * n)(*map(torch.Tensor.data_ptr, tensors)),
+            (_i64 * n)(*map(torch.Tensor.numel, tensors)), (_int * n)(*codes))
+
+
+def _grad_device(grads):
+    return grads[0].device if grads else torch.device('cuda', torch.cuda.current_device())
+
+
+def grad_sumsq(grads):
+    """The sum of the squares of all elements of the tensors: float64 [1] on their device."""
+    who = 'grad_norm'
+    grads = list(grads)
+    ptrs, numel, codes = _tensor_table(grads, who)
+    out = torch.empty(1, dtype=torch.float64, device=_grad_device(grads))
+    ws, nb = _workspace('cflk_grad_workspace_size', (len(grads),), out, who)
+    _check(lib().cflk_grad_sumsq(_stream(), len(grads), ptrs, numel, codes, _ptr(out), _ptr(ws),
+                                 nb), who)
+    return out
+
+
+def clip_grad_norm(grads, max_norm, *, scale=1.0, eps=1e-6, out=None, sumsq=None):
+    """Clip gradients by their global norm: returns norm (float32, no dimensions) = scale * the
+    2-norm of all elements and leaves grads * scale * min(1, max_norm / (norm + eps)) in `out`
+    (default: in place; tensors of the gradients' types or float32). `sumsq` (float64 [1]): the sum
+    of squares to use instead of these tensors' own, as the ranks of a sharded model add it up."""
+    who = 'grad_clip'
+    grads = list(grads)
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads) or any(o.numel() != g.numel() for o, g in zip(outs, grads)):
+        raise ValueError('grad_clip: out must hold a tensor of the same size for each gradient')
+    ptrs, numel, codes = _tensor_table(grads, who)
+    optrs, _, ocodes = (ptrs, numel, codes) if out is None else _tensor_table(outs, who)
+    norm = torch.empty((), dtype=torch.float32, device=_grad_device(grads))
+    if sumsq is not None and (sumsq.dtype != torch.float64 or sumsq.numel() != 1):
+        raise ValueError('grad_clip: sumsq must be one float64')
+    ws, nb = _workspace('cflk_grad_workspace_size', (len(grads),), norm, who)
+    _check(lib().cflk_grad_clip(_stream(), len(grads), ptrs, optrs, numel, codes, ocodes,
+                                _ptr(sumsq), float(max_norm), float(eps), float(scale),
+                                _ptr(norm), _ptr(ws), nb), who)
+    return norm

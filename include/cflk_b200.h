@@ -34,6 +34,7 @@ extern "C" {
 
 #define CFLK_F16 0
 #define CFLK_BF16 1
+#define CFLK_F32 2 /* only where an entry point says so */
 
 /* Message of this thread's last failed call ("" after a successful one). */
 CFLK_API const char* cflk_last_error(void);
@@ -263,6 +264,79 @@ CFLK_API int cflk_volta_opm_outer(void* stream, int dtype, const void* left, con
 CFLK_API int cflk_trimul_contract(void* stream, int dtype, const void* a, const void* b,
                                   float* out, int64_t C, int64_t I, int64_t J, int64_t K,
                                   int incoming);
+
+/* ---- token training (no counterpart in the reference) ---------------------------------- */
+/* What turns token ids into channels, channels into a loss over classes, and what bounds the
+ * gradients before the update. ids and labels are int32 (ids_64 / labels_64 0) or int64 (1). */
+
+/* out[t,:] = scale * table[ids[t],:], a row of zeros for an id outside [0, V). ids [T], table
+ * [V,C], out [T,C]. table_dtype CFLK_F16, CFLK_BF16 or CFLK_F32; out_dtype the same, or any of
+ * the three for a float32 table; the product is taken in float32 and rounded once. Any C;
+ * 16-byte accesses where C % 8 == 0 (C % 4 for float32 to float32) and table and out are 16-byte
+ * aligned, one channel a thread otherwise. */
+CFLK_API int cflk_embed(void* stream, int table_dtype, int out_dtype, int ids_64, const void* ids,
+                        const void* table, void* out, int64_t T, int64_t V, int64_t C,
+                        float scale);
+
+/* The gradient of cflk_embed's table: dtable [V,C] float32, dtable[v,:] = scale * the sum of
+ * dout[t,:] over the tokens t with ids[t] = v (ids outside [0, V) add nowhere); every row is
+ * written. dout [T,C] of dtype CFLK_F16, CFLK_BF16 or CFLK_F32. Tokens are sorted by id and added
+ * in a fixed order in float32: the same bits every run. T and V below 2^31. workspace: at least
+ * cflk_embed_bwd_workspace_size bytes, 256-byte aligned. */
+CFLK_API int cflk_embed_bwd_workspace_size(int64_t T, int64_t V, int64_t C, size_t* bytes);
+CFLK_API int cflk_embed_bwd(void* stream, int dtype, int ids_64, const void* ids,
+                            const void* dout, float* dtable, int64_t T, int64_t V, int64_t C,
+                            float scale, void* workspace, size_t ws_bytes);
+
+/* Softmax cross entropy of a linear layer without keeping its logits l = x w^T + bias: loss[t] =
+ * log(sum_v exp l[t,v]) - l[t, labels[t]] and, in the log2 domain as the attention's, lse[t] =
+ * log2(sum_v exp l[t,v]). x [T,C], w [V,C] 16-bit, bias [V] 16-bit or NULL, loss and lse [T]
+ * float32. A token whose label is outside [0, V) gets loss 0 and lse -inf and its row of x is not
+ * used (it may hold NaN); so does one whose every logit is -inf. C a multiple of 8, any V >= 1;
+ * x and w 16-byte aligned. Products accumulate in float32 (tcgen05). workspace: at least the size
+ * function's bytes, 256-byte aligned. */
+CFLK_API int cflk_linear_xent_workspace_size(int64_t T, int64_t V, int64_t C, size_t* bytes);
+CFLK_API int cflk_linear_xent(void* stream, int dtype, int labels_64, const void* x,
+                              const void* w, const void* bias, const void* labels, float* loss,
+                              float* lse, int64_t T, int64_t V, int64_t C, void* workspace,
+                              size_t ws_bytes);
+
+/* The gradients of cflk_linear_xent for dloss [T] float32 and the forward's lse: with g[t,v] =
+ * dloss[t] (exp(l[t,v]) / sum - [v = labels[t]]), dx [T,C] = g w, dw [V,C] = g^T x and dbias [V]
+ * = sum_t g (16-bit; dbias NULL exactly when bias is). Every row is written: dx is zero for tokens
+ * without a label and for those whose lse is -inf. The logits are computed again, in pieces of
+ * the classes, and g is rounded to the 16-bit type between the products (scaled by a power of
+ * two first, so that float16 keeps its small values); sums are float32 in a fixed order. x, w, dx
+ * and dw 16-byte aligned; workspace as above. */
+CFLK_API int cflk_linear_xent_bwd_workspace_size(int64_t T, int64_t V, int64_t C, size_t* bytes);
+CFLK_API int cflk_linear_xent_bwd(void* stream, int dtype, int labels_64, const void* x,
+                                  const void* w, const void* bias, const void* labels,
+                                  const float* lse, const float* dloss, void* dx, void* dw,
+                                  void* dbias, int64_t T, int64_t V, int64_t C, void* workspace,
+                                  size_t ws_bytes);
+
+/* Gradients as n tensors: host arrays of n device pointers, element counts and types (CFLK_F16,
+ * CFLK_BF16 or CFLK_F32), read during the call only; a tensor may have no elements, and any
+ * alignment its type allows. workspace: at least cflk_grad_workspace_size(n) bytes, 8-byte
+ * aligned; its contents do not matter.
+ *
+ * cflk_grad_sumsq: *sumsq (device, float64) = the sum of the squares of all elements, taken and
+ * added in float64. */
+CFLK_API int cflk_grad_workspace_size(int64_t n, size_t* bytes);
+CFLK_API int cflk_grad_sumsq(void* stream, int64_t n, const void* const* grads,
+                             const int64_t* numel, const int* dtypes, double* sumsq,
+                             void* workspace, size_t ws_bytes);
+
+/* norm = scale * sqrt(sum of squares) and outs = grads * scale * min(1, max_norm / (norm + eps)),
+ * rounded once. scale > 0 takes a loss scale out. outs[i] may be grads[i] (then nothing is moved
+ * when the factor is 1); out_dtypes[i] is dtypes[i], or CFLK_F32 for a buffer of its own. sumsq NULL: the
+ * sum is taken of these tensors; otherwise it is read from the device (the sum of the shards of
+ * several ranks). norm (device, float32) or NULL. A norm that is not finite gives what the
+ * formula gives: zeros and NaN for an infinite one, NaN for NaN. */
+CFLK_API int cflk_grad_clip(void* stream, int64_t n, const void* const* grads, void* const* outs,
+                            const int64_t* numel, const int* dtypes, const int* out_dtypes,
+                            const double* sumsq, float max_norm, float eps, float scale,
+                            float* norm, void* workspace, size_t ws_bytes);
 
 /* ---- diagnostics (no counterpart in the reference) ------------------------------------- */
 
