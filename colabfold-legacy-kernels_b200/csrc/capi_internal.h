@@ -1,6 +1,8 @@
 // Status codes, dtype codes and the last-error message shared by the C-ABI entry points.
 #pragma once
 
+#include <cuda_runtime.h>
+
 #include <cstdint>
 #include <string>
 
@@ -24,12 +26,29 @@ unsigned read_and_clear_status_fused();
 unsigned read_and_clear_status_gemm();
 unsigned read_and_clear_status_opm();
 unsigned read_and_clear_status_xent();
+unsigned read_and_clear_status_head();
 
 // VoltaOpmOuter fused at C = E = 32 (the caller has validated the sizes); the workspace holds
 // wT laid out chunk by chunk (F * 2 KB)
 int opm_outer_fused(void* stream, int dtype, const void* left, const void* right, const void* wT,
                     void* out, int64_t B, int64_t D, int64_t F, void* workspace,
                     size_t ws_bytes);
+
+// The linear softmax cross entropy of heads of few classes (the caller has validated the buffers):
+// whether the sizes fit, its workspace, and the forward or backward
+struct HeadCall {
+    cudaStream_t stream;
+    int dtype, labels_64;
+    const void *x, *w, *bias, *labels;
+    const float *lse_in, *dloss;
+    float *loss, *lse;
+    void *dx, *dw, *dbias;
+    int64_t T, V, C;
+    void* workspace;
+};
+bool xent_head_fits(int64_t V, int64_t C, bool bwd);
+size_t xent_head_workspace(int64_t T, int64_t V, int64_t C, bool bwd);
+cudaError_t xent_head(const HeadCall& c, bool bwd, bool& map_ok);
 
 // VoltaGdp through the tile GEMM (widths the resident-weight row-tile kernel does not take)
 int gdp_general(void* stream, int dtype, const void* x, const void* wp, const void* bp,

@@ -37,41 +37,17 @@
 #include "sm100.cuh"
 #include "tmap.h"
 #include "vec_io.cuh"
+#include "xent_common.cuh"
 
 namespace cflk {
 namespace {
 
 __device__ unsigned g_status;
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kInf = __builtin_huge_valf();
-
 // ------------------------------------------------------------------------------------------
 // the labelled tokens
 // ------------------------------------------------------------------------------------------
 constexpr int kPrepThreads = 256, kPrepItems = 1024;  // tokens a block
-
-template <typename L>
-__device__ __forceinline__ int label_of(const L* labels, long long t, long long V) {
-    const long long l = (long long)labels[t];
-    return l >= 0 && l < V ? (int)l : -1;
-}
-
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-    }
-    return x;
-}
-
-__device__ __forceinline__ int warp_sum(int x) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, d);
-    }
-    return x;
-}
 
 // counts[b]: the block's labelled tokens; maxs[b]: the largest finite |dloss| among them (backward)
 template <typename L>
@@ -110,16 +86,6 @@ __global__ void __launch_bounds__(kPrepThreads)
         counts[blockIdx.x] = s;
         maxs[blockIdx.x] = mm;
     }
-}
-
-// The power of two that brings a positive finite m into [2^13, 2^14); 1 for 0
-__device__ __forceinline__ float grad_scale(float m) {
-    if (!(m > 0.f)) {
-        return 1.f;
-    }
-    int e;
-    frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
-    return exp2f((float)min(14 - e, 126));
 }
 
 struct PrepArgs {
@@ -541,7 +507,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             };
             if constexpr (KIND == kStats) {
                 // log2-domain maximum and sum of this row's columns; -inf where nothing is left
-                float m = -kInf, s = 0.f;
+                float m = -kInf, s = 0.f, at_label = 0.f;
                 const int limit = min(a.vp, a.V - a.v0);
                 for (int ch = 0; ch < 4; ++ch) {
                     const int c0 = col0 + 32 * ch;
@@ -561,37 +527,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                             y[j] += bias_sh[g][32 * ch + j];
                         }
                     }
-                    if (c0 + 32 > limit) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            y[j] = c0 + j < limit ? y[j] : -kInf;
-                        }
-                    }
-                    const int at = lab - c0;
-                    if (at >= 0 && at < 32) {
-                        float z = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            z = j == at ? y[j] : z;
-                        }
-                        a.lab_logit[row + a.row0] = z;
-                    }
-                    float top = y[0];
-#pragma unroll
-                    for (int j = 1; j + 1 < 32; j += 2) {
-                        top = max3(top, y[j], y[j + 1]);
-                    }
-                    top = fmaxf(top, y[31]);
-                    const float m1 = fmaxf(m, top * kLog2e);
-                    const float ref = m1 == -kInf ? 0.f : m1;
-                    float part = 0.f, part1 = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        part += ex2(fmaf(y[j], kLog2e, -ref));
-                        part1 += ex2(fmaf(y[j + 1], kLog2e, -ref));
-                    }
-                    s = s * ex2(m - ref) + (part + part1);
-                    m = m1;
+                    row_stats(y, c0, limit, lab, m, s, at_label);
+                }
+                if (lab >= col0 && lab < min(col0 + 128, limit)) {
+                    a.lab_logit[row + a.row0] = at_label;
                 }
                 const int piece = (it.n0 / PN) * 2 + g;
                 a.part[piece * a.cap + row] = make_float2(m, s);
@@ -620,21 +559,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                                 y[k] += bias_sh[g][64 * j + 32 * h + k];
                             }
                         }
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            y[k] = ex2(fmaf(y[k], kLog2e, -lse2));
-                        }
-                        const int at = lab - c0;
-                        if (at >= 0 && at < 32) {
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) {
-                                y[k] -= k == at ? 1.f : 0.f;
-                            }
-                        }
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            y[k] = dead || c0 + k >= limit ? 0.f : y[k] * dl;
-                        }
+                        row_grad(y, c0, limit, lab, lse2, dl, dead);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             *reinterpret_cast<uint4*>(dst + (((4 * h + q) ^ (r & 7)) << 4)) =
@@ -944,6 +869,7 @@ constexpr size_t kPieceBytes = size_t(512) << 20;  // g of one piece of the clas
 constexpr int kPairs = 74;
 
 struct Plan {
+    bool head;         // few classes: xent_head.cu, whose workspace is all it needs
     int64_t tp;        // rows of the gathered tokens, whole tiles
     int64_t row_step;  // forward: rows a launch
     int64_t vp;        // classes a piece (backward), whole tiles
@@ -962,6 +888,11 @@ bool make_plan(int64_t T, int64_t V, int64_t C, bool bwd, Plan& p) {
     int64_t mul = 0;
     if (__builtin_mul_overflow(T + 256, C * 64, &mul) || __builtin_mul_overflow(V, C * 64, &mul)) {
         return false;
+    }
+    p.head = xent_head_fits(V, C, bwd);
+    if (p.head) {
+        p.bytes = xent_head_workspace(T, V, C, bwd);
+        return true;
     }
     p.tp = (T + PM - 1) / PM * PM;
     const int64_t tiles_v = (V + PN - 1) / PN, tiles_c = (C + PN - 1) / PN, tiles_t = p.tp / PM;
@@ -1062,44 +993,37 @@ bool map3(CUtensorMap* m, const void* p, int64_t slabs, int64_t rows, int64_t co
                         CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-struct Call {
-    cudaStream_t s;
-    int dtype, labels_64;
-    const void *x, *w, *bias, *labels;
-    const float *lse_in, *dloss;
-    float *loss, *lse;
-    void *dx, *dw, *dbias;
-    int64_t T, V, C;
-    uint8_t* ws;
-};
+uint8_t* ws_of(const HeadCall& c) {
+    return static_cast<uint8_t*>(c.workspace);
+}
 
 // label compaction and the gather of x
-cudaError_t prepare(const Call& c, const Plan& p) {
+cudaError_t prepare(const HeadCall& c, const Plan& p) {
     const int64_t nb = (c.T + kPrepItems - 1) / kPrepItems;
     PrepArgs a{};
     a.dloss = c.dloss;
     a.lse = c.lse_in;
     a.loss = c.loss;
     a.lse_out = c.lse;
-    a.counts = reinterpret_cast<int*>(c.ws + p.counts);
-    a.maxs = reinterpret_cast<float*>(c.ws + p.maxs);
+    a.counts = reinterpret_cast<int*>(ws_of(c) + p.counts);
+    a.maxs = reinterpret_cast<float*>(ws_of(c) + p.maxs);
     a.T = (int)c.T;
     a.nblocks = (int)nb;
     a.V = c.V;
-    a.perm = reinterpret_cast<int*>(c.ws + p.perm);
-    a.lab = reinterpret_cast<int*>(c.ws + p.lab);
-    a.lse_c = reinterpret_cast<float*>(c.ws + p.lse_c);
-    a.dl_c = reinterpret_cast<float*>(c.ws + p.dl_c);
-    a.count = reinterpret_cast<int*>(c.ws + p.scalars);
-    a.inv = reinterpret_cast<float*>(c.ws + p.scalars + 4);
-    int* counts = reinterpret_cast<int*>(c.ws + p.counts);
-    float* maxs = reinterpret_cast<float*>(c.ws + p.maxs);
+    a.perm = reinterpret_cast<int*>(ws_of(c) + p.perm);
+    a.lab = reinterpret_cast<int*>(ws_of(c) + p.lab);
+    a.lse_c = reinterpret_cast<float*>(ws_of(c) + p.lse_c);
+    a.dl_c = reinterpret_cast<float*>(ws_of(c) + p.dl_c);
+    a.count = reinterpret_cast<int*>(ws_of(c) + p.scalars);
+    a.inv = reinterpret_cast<float*>(ws_of(c) + p.scalars + 4);
+    int* counts = reinterpret_cast<int*>(ws_of(c) + p.counts);
+    float* maxs = reinterpret_cast<float*>(ws_of(c) + p.maxs);
     const auto run = [&](auto tag) {
         using L = decltype(tag);
         const L* labels = static_cast<const L*>(c.labels);
-        xent_count_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.s>>>(labels, c.dloss, (int)c.T,
+        xent_count_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.stream>>>(labels, c.dloss, (int)c.T,
                                                                      c.V, counts, maxs);
-        xent_compact_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.s>>>(labels, a);
+        xent_compact_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.stream>>>(labels, a);
     };
     if (c.labels_64) {
         run((long long)0);
@@ -1107,41 +1031,41 @@ cudaError_t prepare(const Call& c, const Plan& p) {
         run(0);
     }
     const unsigned grid = (unsigned)std::min<int64_t>((c.T + 63 + 7) / 8, 148 * 8);
-    xent_gather_kernel<<<grid, 256, 0, c.s>>>(static_cast<const uint4*>(c.x), a.perm, a.count,
-                                              reinterpret_cast<uint4*>(c.ws + p.xc),
+    xent_gather_kernel<<<grid, 256, 0, c.stream>>>(static_cast<const uint4*>(c.x), a.perm, a.count,
+                                              reinterpret_cast<uint4*>(ws_of(c) + p.xc),
                                               (int)(c.C / 8));
     return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t forward(const Call& c, const Plan& p, bool& map_ok) {
+cudaError_t forward(const HeadCall& c, const Plan& p, bool& map_ok) {
     const CUtensorMapDataType t =
         c.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap tx, tw;
-    map_ok = map2(&tx, t, 2, c.ws + p.xc, p.tp, c.C, 128) && map2(&tw, t, 2, c.w, c.V, c.C, 128);
+    map_ok = map2(&tx, t, 2, ws_of(c) + p.xc, p.tp, c.C, 128) && map2(&tw, t, 2, c.w, c.V, c.C, 128);
     if (!map_ok) {
         return cudaSuccess;
     }
     cudaError_t e = prepare(c, p);
     GemmArgs a{};
-    a.count = reinterpret_cast<int*>(c.ws + p.scalars);
+    a.count = reinterpret_cast<int*>(ws_of(c) + p.scalars);
     a.V = (int)c.V;
     a.C = (int)c.C;
     a.vp = (int)((c.V + PN - 1) / PN * PN);
     a.splits = 1;
     a.cap = p.row_step;
-    a.lab = reinterpret_cast<int*>(c.ws + p.lab);
+    a.lab = reinterpret_cast<int*>(ws_of(c) + p.lab);
     a.bias = c.bias;
-    a.part = reinterpret_cast<float2*>(c.ws + p.part);
-    a.lab_logit = reinterpret_cast<float*>(c.ws + p.lab_logit);
+    a.part = reinterpret_cast<float2*>(ws_of(c) + p.part);
+    a.lab_logit = reinterpret_cast<float*>(ws_of(c) + p.lab_logit);
     for (int64_t r0 = 0; e == cudaSuccess && r0 < c.T; r0 += p.row_step) {
         a.row0 = (int)r0;
         a.rows = (int)std::min(p.row_step, c.T - r0);
         const int64_t items = (int64_t)((a.rows + PM - 1) / PM) * (a.vp / PN);
-        e = launch_gemm<T, kStats>(c.s, tx, tw, tw, a, items);
+        e = launch_gemm<T, kStats>(c.stream, tx, tw, tw, a, items);
         if (e == cudaSuccess) {
-            xent_join_kernel<<<(a.rows + 31) / 32, 256, 0, c.s>>>(
-                a.part, a.lab_logit, reinterpret_cast<int*>(c.ws + p.perm), a.count, a.row0, a.rows,
+            xent_join_kernel<<<(a.rows + 31) / 32, 256, 0, c.stream>>>(
+                a.part, a.lab_logit, reinterpret_cast<int*>(ws_of(c) + p.perm), a.count, a.row0, a.rows,
                 a.cap, 2 * (a.vp / PN), c.loss, c.lse);
             e = cudaGetLastError();
         }
@@ -1150,19 +1074,19 @@ cudaError_t forward(const Call& c, const Plan& p, bool& map_ok) {
 }
 
 template <typename T>
-cudaError_t backward(const Call& c, const Plan& p, bool& map_ok) {
+cudaError_t backward(const HeadCall& c, const Plan& p, bool& map_ok) {
     const CUtensorMapDataType t =
         c.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    T* g = reinterpret_cast<T*>(c.ws + p.g);
-    float* dx_acc = reinterpret_cast<float*>(c.ws + p.dx_acc);
-    float* dw_acc = reinterpret_cast<float*>(c.ws + p.dw_acc);
-    float* db_part = reinterpret_cast<float*>(c.ws + p.db_part);
-    const float* inv = reinterpret_cast<float*>(c.ws + p.scalars + 4);
+    T* g = reinterpret_cast<T*>(ws_of(c) + p.g);
+    float* dx_acc = reinterpret_cast<float*>(ws_of(c) + p.dx_acc);
+    float* dw_acc = reinterpret_cast<float*>(ws_of(c) + p.dw_acc);
+    float* db_part = reinterpret_cast<float*>(ws_of(c) + p.db_part);
+    const float* inv = reinterpret_cast<float*>(ws_of(c) + p.scalars + 4);
     // K-major operands in boxes of 128 rows, MN-major ones in boxes of 64 K rows
     CUtensorMap x_k, w_k, g_k, x_n, w_n, g_m, g_out, dx_out, dw_out;
-    map_ok = map2(&x_k, t, 2, c.ws + p.xc, p.tp, c.C, 128) &&
+    map_ok = map2(&x_k, t, 2, ws_of(c) + p.xc, p.tp, c.C, 128) &&
              map2(&w_k, t, 2, c.w, c.V, c.C, 128) && map2(&g_k, t, 2, g, p.tp, p.vp, 128) &&
-             map2(&x_n, t, 2, c.ws + p.xc, p.tp, c.C, 64) && map2(&w_n, t, 2, c.w, c.V, c.C, 64) &&
+             map2(&x_n, t, 2, ws_of(c) + p.xc, p.tp, c.C, 64) && map2(&w_n, t, 2, c.w, c.V, c.C, 64) &&
              map2(&g_m, t, 2, g, p.tp, p.vp, 64) && map3(&dx_out, dx_acc, p.dx_splits, p.tp, c.C) &&
              (p.dw_splits > 1 ? map3(&dw_out, dw_acc, p.dw_splits, p.vp, c.C)
                               : map2(&dw_out, t, 2, c.dw, c.V, c.C, 128));
@@ -1172,14 +1096,14 @@ cudaError_t backward(const Call& c, const Plan& p, bool& map_ok) {
     g_out = g_k;
     cudaError_t e = prepare(c, p);
     GemmArgs a{};
-    a.count = reinterpret_cast<int*>(c.ws + p.scalars);
+    a.count = reinterpret_cast<int*>(ws_of(c) + p.scalars);
     a.V = (int)c.V;
     a.C = (int)c.C;
     a.vp = (int)p.vp;
-    a.lab = reinterpret_cast<int*>(c.ws + p.lab);
+    a.lab = reinterpret_cast<int*>(ws_of(c) + p.lab);
     a.bias = c.bias;
-    a.lse_c = reinterpret_cast<float*>(c.ws + p.lse_c);
-    a.dl_c = reinterpret_cast<float*>(c.ws + p.dl_c);
+    a.lse_c = reinterpret_cast<float*>(ws_of(c) + p.lse_c);
+    a.dl_c = reinterpret_cast<float*>(ws_of(c) + p.dl_c);
     a.inv = inv;
     const int64_t tiles_t = p.tp / PM, tiles_c = (c.C + PN - 1) / PN;
     for (int64_t v0 = 0; e == cudaSuccess && v0 < c.V; v0 += p.vp) {
@@ -1187,30 +1111,30 @@ cudaError_t backward(const Call& c, const Plan& p, bool& map_ok) {
         const int64_t classes = std::min(p.vp, c.V - v0);
         const int64_t tiles_p = (classes + PN - 1) / PN;
         a.splits = 1;
-        e = launch_gemm<T, kGrad>(c.s, x_k, w_k, g_out, a, tiles_t * tiles_p);
+        e = launch_gemm<T, kGrad>(c.stream, x_k, w_k, g_out, a, tiles_t * tiles_p);
         if (e == cudaSuccess && c.dbias != nullptr) {
-            xent_colsum_kernel<T><<<dim3((unsigned)tiles_p, kBiasChunks), 256, 0, c.s>>>(
+            xent_colsum_kernel<T><<<dim3((unsigned)tiles_p, kBiasChunks), 256, 0, c.stream>>>(
                 g, a.count, a.vp, (int)classes, db_part);
-            xent_dbias_kernel<T><<<(unsigned)tiles_p, 256, 0, c.s>>>(
+            xent_dbias_kernel<T><<<(unsigned)tiles_p, 256, 0, c.stream>>>(
                 db_part, a.vp, (int)classes, inv, static_cast<T*>(c.dbias) + v0);
             e = cudaGetLastError();
         }
         if (e == cudaSuccess) {
             a.splits = p.dx_splits;
             a.accumulate = v0 > 0;
-            e = launch_gemm<T, kDx>(c.s, g_k, w_n, dx_out, a, tiles_t * tiles_c * a.splits);
+            e = launch_gemm<T, kDx>(c.stream, g_k, w_n, dx_out, a, tiles_t * tiles_c * a.splits);
         }
         if (e == cudaSuccess) {
             a.splits = p.dw_splits;
             const int64_t items = tiles_p * tiles_c * a.splits;
             if (p.dw_splits == 1) {
-                e = launch_gemm<T, kDw>(c.s, g_m, x_n, dw_out, a, items);
+                e = launch_gemm<T, kDw>(c.stream, g_m, x_n, dw_out, a, items);
             } else {
-                e = launch_gemm<T, kDwSlab>(c.s, g_m, x_n, dw_out, a, items);
+                e = launch_gemm<T, kDwSlab>(c.stream, g_m, x_n, dw_out, a, items);
                 if (e == cudaSuccess) {
                     const int64_t total8 = classes * c.C / 8;
                     xent_dw_kernel<T><<<(unsigned)std::min<int64_t>((total8 + 255) / 256, 148 * 8),
-                                        256, 0, c.s>>>(dw_acc, p.vp * c.C, a.splits, inv,
+                                        256, 0, c.stream>>>(dw_acc, p.vp * c.C, a.splits, inv,
                                                        static_cast<T*>(c.dw) + v0 * c.C, total8);
                     e = cudaGetLastError();
                 }
@@ -1218,8 +1142,8 @@ cudaError_t backward(const Call& c, const Plan& p, bool& map_ok) {
         }
     }
     if (e == cudaSuccess) {
-        xent_dx_kernel<T><<<(unsigned)std::min<int64_t>((c.T + 7) / 8, 148 * 8), 256, 0, c.s>>>(
-            dx_acc, p.tp * c.C, p.dx_splits, reinterpret_cast<int*>(c.ws + p.perm), a.count, inv,
+        xent_dx_kernel<T><<<(unsigned)std::min<int64_t>((c.T + 7) / 8, 148 * 8), 256, 0, c.stream>>>(
+            dx_acc, p.tp * c.C, p.dx_splits, reinterpret_cast<int*>(ws_of(c) + p.perm), a.count, inv,
             static_cast<T*>(c.dx), (int)c.T, (int)c.C);
         e = cudaGetLastError();
     }
@@ -1272,7 +1196,7 @@ int finish(const char* who, bool map_ok, cudaError_t e) {
 }
 
 int check_workspace(const char* who, const void* ws, size_t have, size_t need) {
-    if (ws == nullptr || have < need || reinterpret_cast<uintptr_t>(ws) % 256 != 0) {
+    if ((ws == nullptr && need > 0) || have < need || reinterpret_cast<uintptr_t>(ws) % 256 != 0) {
         return fail(kInvalidArgument,
                     std::string(who) + ": workspace below the size function's or not 256-byte "
                                        "aligned");
@@ -1322,8 +1246,8 @@ extern "C" int cflk_linear_xent(void* stream, int dtype, int labels_64, const vo
     if (rc != kOk) {
         return rc;
     }
-    Call c{};
-    c.s = static_cast<cudaStream_t>(stream);
+    HeadCall c{};
+    c.stream = static_cast<cudaStream_t>(stream);
     c.dtype = dtype;
     c.labels_64 = labels_64;
     c.x = x;
@@ -1335,10 +1259,11 @@ extern "C" int cflk_linear_xent(void* stream, int dtype, int labels_64, const vo
     c.T = T;
     c.V = V;
     c.C = C;
-    c.ws = static_cast<uint8_t*>(workspace);
+    c.workspace = workspace;
     bool map_ok = true;
-    const cudaError_t e =
-        dtype == kBF16 ? forward<__nv_bfloat16>(c, p, map_ok) : forward<__half>(c, p, map_ok);
+    const cudaError_t e = p.head           ? xent_head(c, false, map_ok)
+                          : dtype == kBF16 ? forward<__nv_bfloat16>(c, p, map_ok)
+                                           : forward<__half>(c, p, map_ok);
     return finish(who, map_ok, e);
 }
 
@@ -1386,8 +1311,8 @@ extern "C" int cflk_linear_xent_bwd(void* stream, int dtype, int labels_64, cons
     if (rc != kOk) {
         return rc;
     }
-    Call c{};
-    c.s = s;
+    HeadCall c{};
+    c.stream = s;
     c.dtype = dtype;
     c.labels_64 = labels_64;
     c.x = x;
@@ -1402,9 +1327,10 @@ extern "C" int cflk_linear_xent_bwd(void* stream, int dtype, int labels_64, cons
     c.T = T;
     c.V = V;
     c.C = C;
-    c.ws = static_cast<uint8_t*>(workspace);
+    c.workspace = workspace;
     bool map_ok = true;
-    const cudaError_t e =
-        dtype == kBF16 ? backward<__nv_bfloat16>(c, p, map_ok) : backward<__half>(c, p, map_ok);
+    const cudaError_t e = p.head           ? xent_head(c, true, map_ok)
+                          : dtype == kBF16 ? backward<__nv_bfloat16>(c, p, map_ok)
+                                           : backward<__half>(c, p, map_ok);
     return finish(who, map_ok, e);
 }

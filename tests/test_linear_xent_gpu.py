@@ -106,7 +106,8 @@ def close(got, want):
 @pytest.mark.parametrize('T,V,C', [
     (1, 1, 8), (1, 23, 256), (1, 1000, 64), (3, 2, 8), (5, 64, 128), (64, 23, 24), (127, 50, 384),
     (128, 128, 128), (129, 129, 136), (255, 21, 72), (256, 256, 256), (257, 257, 264),
-    (300, 513, 64), (513, 64, 520), (700, 1000, 40), (1100, 300, 16), (1025, 22, 256)])
+    (300, 513, 64), (513, 64, 520), (700, 1000, 40), (1100, 300, 16), (1025, 22, 256),
+    (20000, 23, 256), (19500, 70, 128), (300, 100, 200), (300, 40, 392)])
 def test_linear_xent(T, V, C, dt, cuda_device):
     for bias in (True, False):
         p = problem(T, V, C, dt, bias=bias)
@@ -210,7 +211,7 @@ def reference64(x, w, labels, dloss, bias):
     (5000, 70001, 64, 'bf16', .9),   # classes in several pieces
     (2100, 140003, 40, 'f16', 1.0),
     (300000, 23, 64, 'bf16', .15), (200001, 64, 128, 'f16', .9), (50003, 100, 256, 'bf16', 1.0),
-    (20001, 129, 72, 'bf16', .5), (9, 33000, 1032, 'f16', 1.0)])
+    (20001, 129, 72, 'bf16', .5), (700001, 23, 16, 'f16', .3), (9, 33000, 1032, 'f16', 1.0)])
 def test_large(T, V, C, dt, labelled, cuda_device):
     """Relative 2-norms against float64: the inputs' products in 16 bits leave u / sqrt(3) or so in
     g and the same again in the outputs; 2 u bounds their sum with room for the float32 sums."""

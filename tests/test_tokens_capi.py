@@ -75,8 +75,8 @@ def xent_bwd(dt=1, l64=0, x=P, w=P, b=Z, lab=P, lse=P, dl=P, dx=P, dw=P, db=Z, T
 
 
 BAD = [dict(dt=2), dict(l64=2), dict(T=-1), dict(V=0), dict(C=0), dict(C=12), dict(T=1 << 31),
-       dict(V=1 << 31), dict(x=Z), dict(w=Z), dict(lab=Z), dict(lse=Z), dict(ws=Z), dict(n=16),
-       dict(ws=ctypes.c_void_p(16)), dict(x=ctypes.c_void_p(8)), dict(w=ctypes.c_void_p(8))]
+       dict(V=1 << 31), dict(x=Z), dict(w=Z), dict(lab=Z), dict(lse=Z), dict(ws=Z, V=500), dict(n=16, V=500),
+       dict(ws=ctypes.c_void_p(16), V=500), dict(x=ctypes.c_void_p(8)), dict(w=ctypes.c_void_p(8))]
 
 
 @pytest.mark.parametrize('bad', BAD + [dict(loss=Z)])
