@@ -8,10 +8,9 @@
 //
 //   * a persistent CTA an SM; it lists its labelled tokens in shared memory (blocks of 128 tokens
 //     in turn over the CTAs) and works through them 128 at a time, so positions without a label
-//     cost nothing but dx's zeros, which two idle warps write;
+//     cost nothing but dx's zeros, which a warp sends as bulk copies;
 //   * w stays in shared memory in one layout that serves as the K-major B of the logits and the
-//     N-major B of dx; a tile of x, gathered row by row (TMA gather of four rows an instruction),
-//     is the K-major A of the logits, then the N-major B of dw, then the staging of dx, whose rows
+//     N-major B of dx; a tile of x, gathered row by row by four warps' asynchronous copies, is the K-major A of the logits, then the N-major B of dw, then the staging of dx, whose rows
 //     leave in whole lines; g is the K-major A of dx and the M-major A of dw;
 //   * two warpgroups take the tiles in turn, each with its own tensor-memory slot, so one's
 //     exponentials overlap the other's products and stores; one warp issues all MMAs in a fixed
@@ -42,8 +41,9 @@ namespace {
 
 __device__ unsigned g_status;
 
-constexpr int kThreads = 384;         // TMA, MMA, two zeroing warps; two warpgroups of workers
-constexpr int kWorker0 = 4;
+// two warpgroups of workers, then the zeroing, the MMA and four loading warps
+constexpr int kThreads = 448;
+constexpr int kZeroWarp = 8, kMmaWarp = 9, kLoad0 = 10, kLoaders = 4;
 constexpr int kRoundBlocks = 32;      // blocks of 128 tokens a CTA lists at a time
 constexpr int kRound = kRoundBlocks * 128;
 constexpr int kAtom = 128 * 128;      // 128 rows of 64 16-bit columns, 128-byte swizzle
@@ -81,6 +81,7 @@ bool make_layout(int64_t V, int64_t C, bool bwd, Layout& l) {
 }
 
 struct HeadArgs {
+    const void* x;
     const void* labels;
     const void* bias;
     const float* dloss;  // backward, with lse_in
@@ -94,13 +95,20 @@ struct HeadArgs {
     Layout l;
 };
 
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint64_t* bar,
-                                            int col, int r0, int r1, int r2, int r3) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-        "l"(map), "r"(col), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
-        : "memory");
+// 16 bytes from global to shared memory, zeros where `bytes` is 0
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_wait_all() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// `bytes` (a multiple of 16) from shared to global memory, both 16-byte aligned
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+                 "r"(src), "r"(bytes)
+                 : "memory");
 }
 
 // whether the phase with the given parity is complete
@@ -118,8 +126,7 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 
 template <typename T, typename L, bool BWD>
 __global__ void __launch_bounds__(kThreads, 1)
-    head_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
-                const __grid_constant__ HeadArgs a) {
+    head_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ HeadArgs a) {
     using E = Elem<T>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -129,6 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint32_t tmem_sh;
     __shared__ int abort_flag;
     __shared__ float bias_sh[128];
+    __shared__ __align__(16) uint4 zero_sh[32];
     __shared__ int block_count[kRoundBlocks + 1];
     __shared__ float max_sh[kThreads / 32];
 
@@ -149,11 +157,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         return (((long long)rd * kRoundBlocks + i) * gridDim.x + blockIdx.x) * 128 + j;
     };
 
-    if (warp == 1) {
+    if (warp == kMmaWarp) {
         if (lane == 0) {
             mbar_init(&w_full, 1);
             for (int i = 0; i < 4; ++i) {
-                mbar_init(&x_full[i], 1);
+                mbar_init(&x_full[i], 32 * kLoaders / l.nx);  // the loading warps' lanes
                 mbar_init(&x_free[i], BWD ? 128 : 1);
             }
             for (int i = 0; i < 2; ++i) {
@@ -169,6 +177,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         tmem_alloc(&tmem_sh, 512);
         tmem_relinquish();
+    }
+    if (warp == kZeroWarp) {
+        zero_sh[lane] = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
     }
     if (threadIdx.x < 128) {
         bias_sh[threadIdx.x] = a.bias != nullptr && (int)threadIdx.x < a.V
@@ -207,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = tmem_sh;
     const uint32_t dw_col = tmem + 256;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == kZeroWarp && lane == 0) {
         mbar_arrive_expect_tx(&w_full, l.atoms * l.vp * 128);
         for (int i = 0; i < l.atoms; ++i) {
             tma_load_2d(smem + i * l.vp * 128, &tw, &w_full, 64 * i, 0);
@@ -222,15 +234,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int rd = 0; rd < rounds; ++rd) {
         // list this round's tokens: the labelled ones in order from the front, the others from
         // the back
-        for (int i = warp; i < kRoundBlocks; i += kThreads / 32) {
+        constexpr int kMine = (kRoundBlocks * 32 + kThreads - 1) / kThreads;  // blocks a warp
+        unsigned ballots[kMine][4];
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            const int i = warp + k * (kThreads / 32);
             int n = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const long long t = token(rd, i, 32 * j + lane);
-                n += __popc(__ballot_sync(0xffffffffu,
-                                          t < a.T && label_of(labels, t, a.V) >= 0));
+                const long long t = i < kRoundBlocks ? token(rd, i, 32 * j + lane) : a.T;
+                ballots[k][j] =
+                    __ballot_sync(0xffffffffu, t < a.T && label_of(labels, t, a.V) >= 0);
+                n += __popc(ballots[k][j]);
             }
-            if (lane == 0) {
+            if (lane == 0 && i < kRoundBlocks) {
                 block_count[i] = n;
             }
         }
@@ -250,19 +267,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncthreads();
-        for (int i = warp; i < kRoundBlocks; i += kThreads / 32) {
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            const int i = warp + k * (kThreads / 32);
+            if (i >= kRoundBlocks) {
+                break;
+            }
             int at = block_count[i];
-            // unlisted tokens before this block: those of whole blocks
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const long long t = token(rd, i, 32 * j + lane);
-                const bool in = t < a.T, lab = in && label_of(labels, t, a.V) >= 0;
-                const unsigned ballot = __ballot_sync(0xffffffffu, lab);
+                const unsigned ballot = ballots[k][j];
                 const int before = at + __popc(ballot & ((1u << lane) - 1));
-                if (lab) {
+                if ((ballot >> lane) & 1) {
                     list[before] = (int)t;
                 } else {
                     // token 128 i + 32 j + lane of the round, `before` of them labelled
+                    const bool in = t < a.T;
                     list[kRound - 1 - (128 * i + 32 * j + lane - before)] = in ? (int)t : -1;
                     if (!BWD && in) {
                         a.loss[t] = 0.f;
@@ -276,34 +297,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int count = block_count[kRoundBlocks];
         const int n = (count + 127) / 128;
 
-        if (warp == 0) {
-            // gather: lane i brings rows 4 i .. 4 i + 3 of the tile, 64 columns an instruction;
-            // the last tile's missing rows repeat the last token (their g is zero)
-            for (int c = 0; ok && c < n; ++c) {
-                const int g = base + c, b = g % l.nx;
-                // lane 0 waits for all, so that the warp stays together
+        if (warp >= kLoad0) {
+            // the labelled rows of x, 16 bytes a copy, 8, 16 or 32 lanes a row; the last tile's
+            // missing rows repeat the last token (their g is zero). Each tile buffer has its
+            // own one or two warps, so as many tiles are under way as there are buffers.
+            const int wpt = kLoaders / l.nx, b = (warp - kLoad0) / wpt;  // warps a tile, buffer
+            const int part = (warp - kLoad0) % wpt, rows = 128 / wpt;
+            const int lpr = cn <= 64 ? 8 : cn <= 128 ? 16 : 32, rpw = 32 / lpr;
+            const int piece = lane & (lpr - 1), sub = lane / lpr;
+            const bool on = piece * 8 < cn;
+            const uint32_t bytes = piece * 8 < a.C ? 16 : 0;  // zeros up to the K step
+            const T* x = static_cast<const T*>(a.x) + (bytes ? piece * 8 : 0);
+            const uint32_t dst = smem_u32(xs + b * xbytes) + (piece >> 3) * kAtom;
+            // tiles g = base + c with g % nx == b
+            for (int c = (b - base % l.nx + l.nx) % l.nx; c < n; c += l.nx) {
+                const int g = base + c;
                 if (lane == 0) {
                     ok = g < l.nx || mbar_wait(&x_free[b], (g / l.nx - 1) & 1, &g_status,
                                                kStatusSyncWait, &abort_flag);
-                    if (ok) {
-                        mbar_arrive_expect_tx(&x_full[b], xbytes);
-                    }
                 }
                 ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
                 if (!ok) {
                     break;
                 }
-                int r[4];
+                for (int i = part * rows + sub; i < (part + 1) * rows; i += 8 * rpw) {
+                    int t[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    r[i] = list[min(c * 128 + 4 * lane + i, count - 1)];
+                    for (int u = 0; u < 8; ++u) {
+                        t[u] = list[min(c * 128 + i + u * rpw, count - 1)];
+                    }
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const int row = i + u * rpw;
+                        if (on) {
+                            copy16(dst + row * 128 + (((piece & 7) ^ (row & 7)) << 4),
+                                   x + (long long)t[u] * a.C, bytes);
+                        }
+                    }
                 }
-                const uint32_t dst = smem_u32(xs + b * xbytes) + lane * 512;
-                for (int i = 0; i < l.atoms; ++i) {
-                    tma_gather4(dst + i * kAtom, &tx, &x_full[b], 64 * i, r[0], r[1], r[2], r[3]);
-                }
+                copy_wait_all();
+                fence_async_smem();
+                mbar_arrive(&x_full[b]);
             }
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == kMmaWarp && lane == 0) {
             const uint32_t sw = smem_u32(smem);
             const uint32_t id_l = idesc_f16(E::kBf16, 128, vn, false, false);
             const auto k_major = [](uint32_t at) { return smem_desc(at, 16, 1024, kSwizzle128B); };
@@ -418,18 +454,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-        } else if (BWD && (warp == 2 || warp == 3)) {
-            // zeros for the rows without a label: a warp a row
-            const int rest = kRound - count, cv = a.C / 8;
-            for (int i = warp - 2; i < rest; i += 2) {
+        } else if (BWD && warp == kZeroWarp) {
+            // zeros for the rows without a label: a bulk copy of a zeroed row each
+            for (int i = lane; i < kRound - count; i += 32) {
                 const int t = list[kRound - 1 - i];
-                if (t >= 0 && lane < cv) {
-                    reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + (long long)t * a.C)[lane] =
-                        make_uint4(0, 0, 0, 0);
+                if (t >= 0) {
+                    bulk_store(static_cast<T*>(a.dx) + (long long)t * a.C, smem_u32(zero_sh),
+                               a.C * 2);
                 }
             }
-        } else if (warp >= kWorker0) {
-            const int h = (warp - kWorker0) >> 2;          // warpgroup
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        } else if (warp < kZeroWarp) {
+            const int h = warp >> 2;                       // warpgroup
             const int r = ((warp & 3) << 5) | lane;        // row of the tile, tensor-memory lane
             const uint32_t slot = tmem + 128 * h + tmem_lane_base(warp);
             for (int c = (base + h) & 1; c < n; c += 2) {
@@ -564,16 +600,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
     }
     // every copy has landed and every MMA is done before shared and tensor memory go
-    if (warp == 0 && lane == 0) {
+    if (warp == kZeroWarp && lane == 0) {
         mbar_wait(&w_full, 0, &g_status, kStatusTmaWait, nullptr, kDrainLimitNs);
-        if (abort_flag) {
-            for (int g = max(0, base - l.nx); g < base; ++g) {
-                mbar_wait(&x_full[g % l.nx], (g / l.nx) & 1, &g_status, kStatusTmaWait, nullptr,
-                          kDrainLimitNs);
-            }
-        }
     }
-    if (warp == 1 && lane == 0) {
+    if (BWD && warp == kZeroWarp) {
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    if (warp == kMmaWarp && lane == 0) {
         mma_commit(&drain);
         mbar_wait(&drain, 0, &g_status, kStatusMmaWait, nullptr, kDrainLimitNs);
     }
@@ -583,8 +616,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     if constexpr (BWD) {
         float* db_sh = reinterpret_cast<float*>(list);  // [warp of the workers][128]
-        if (warp >= kWorker0) {
-            const int h = (warp - kWorker0) >> 2, w = warp & 3;
+        if (warp < kZeroWarp) {
+            const int h = warp >> 2, w = warp & 3;
             // dw: lane = class; with 64 rows lanes 32 w + i (i < 16) hold class 16 w + i
             const int v = l.vp == 128 ? 32 * w + lane : 16 * w + lane;
             const bool mine = v < a.V && (l.vp == 128 || lane < 16);
@@ -631,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 1) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -697,8 +730,7 @@ int head_grid(int64_t T) {
 }
 
 template <typename T, typename L, bool BWD>
-cudaError_t launch(const HeadCall& c, const CUtensorMap& tx, const CUtensorMap& tw,
-                   const HeadArgs& a) {
+cudaError_t launch(const HeadCall& c, const CUtensorMap& tw, const HeadArgs& a) {
     auto kern = head_kernel<T, L, BWD>;
     static bool done[kMaxDevices] = {};
     int dev = 0;
@@ -715,7 +747,7 @@ cudaError_t launch(const HeadCall& c, const CUtensorMap& tx, const CUtensorMap& 
             done[dev] = true;
         }
     }
-    kern<<<head_grid(c.T), kThreads, a.l.bytes, c.stream>>>(tx, tw, a);
+    kern<<<head_grid(c.T), kThreads, a.l.bytes, c.stream>>>(tw, a);
     return cudaGetLastError();
 }
 
@@ -733,6 +765,7 @@ size_t xent_head_workspace(int64_t T, int64_t V, int64_t C, bool bwd) {
 cudaError_t xent_head(const HeadCall& c, bool bwd, bool& map_ok) {
     HeadArgs a{};
     make_layout(c.V, c.C, bwd, a.l);
+    a.x = c.x;
     a.labels = c.labels;
     a.bias = c.bias;
     a.dloss = c.dloss;
@@ -748,23 +781,21 @@ cudaError_t xent_head(const HeadCall& c, bool bwd, bool& map_ok) {
     a.db_part = a.dw_part + (size_t)grid * c.V * c.C;
     const CUtensorMapDataType t =
         c.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    CUtensorMap tx, tw;
-    const uint64_t dx[2] = {(uint64_t)c.C, (uint64_t)c.T}, dw[2] = {(uint64_t)c.C, (uint64_t)c.V};
-    const uint64_t st[1] = {(uint64_t)c.C};
-    const uint32_t bx[2] = {64, 1}, bw[2] = {64, (uint32_t)a.l.vp};
-    map_ok = encode_tiled(&tx, t, 2, 2, c.x, dx, st, bx, CU_TENSOR_MAP_SWIZZLE_128B) &&
-             encode_tiled(&tw, t, 2, 2, c.w, dw, st, bw, CU_TENSOR_MAP_SWIZZLE_128B);
+    CUtensorMap tw;
+    const uint64_t dw[2] = {(uint64_t)c.C, (uint64_t)c.V}, st[1] = {(uint64_t)c.C};
+    const uint32_t bw[2] = {64, (uint32_t)a.l.vp};
+    map_ok = encode_tiled(&tw, t, 2, 2, c.w, dw, st, bw, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!map_ok) {
         return cudaSuccess;
     }
     const auto run = [&](auto tag) -> cudaError_t {
         using T = decltype(tag);
         if (!bwd) {
-            return c.labels_64 ? launch<T, long long, false>(c, tx, tw, a)
-                               : launch<T, int, false>(c, tx, tw, a);
+            return c.labels_64 ? launch<T, long long, false>(c, tw, a)
+                               : launch<T, int, false>(c, tw, a);
         }
-        cudaError_t e = c.labels_64 ? launch<T, long long, true>(c, tx, tw, a)
-                                    : launch<T, int, true>(c, tx, tw, a);
+        cudaError_t e = c.labels_64 ? launch<T, long long, true>(c, tw, a)
+                                    : launch<T, int, true>(c, tw, a);
         if (e == cudaSuccess) {
             const int blocks = (a.V * a.C / 4 + 31) / 32 + (c.bias != nullptr ? (a.V + 31) / 32 : 0);
             head_reduce_kernel<T><<<blocks, 256, 0, c.stream>>>(
