@@ -476,15 +476,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             const int buf = lt & 1;
             const int row = it.m0 + 128 * (int)rank + r;  // of the launch's rows
             const int col0 = it.n0 + 128 * g;
-            [[maybe_unused]] int lab = INT_MIN / 2;  // relative to the piece; no token
-            [[maybe_unused]] float lse2 = 0.f, dl = 0.f;
+            [[maybe_unused]] int lab = INT_MIN / 2;  // no token
+            [[maybe_unused]] GradRow grad;
+            grad.kill();
             if constexpr (KIND == kStats || KIND == kGrad) {
                 const int tok = row + (KIND == kStats ? a.row0 : 0);
                 if (tok < n) {
                     lab = a.lab[tok] - a.v0;
-                    if constexpr (KIND == kGrad) {
-                        lse2 = a.lse_c[tok];
-                        dl = a.dl_c[tok];
+                    if (KIND == kGrad && a.lse_c[tok] > -kInf) {
+                        grad.lse2 = a.lse_c[tok];
+                        grad.dl = a.dl_c[tok];
+                        grad.label = lab;
                     }
                 }
                 if (a.bias != nullptr) {
@@ -536,7 +538,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 a.part[piece * a.cap + row] = make_float2(m, s);
             } else if constexpr (KIND == kGrad) {
                 const int limit = min(a.vp, a.V - a.v0);
-                const bool dead = lse2 == -kInf || lab == INT_MIN / 2;  // nothing left, or no token
                 for (int j = 0; j < 2; ++j) {
                     const int b0 = col0 + 64 * j;
                     if (b0 >= limit) {
@@ -549,17 +550,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                         uint32_t v[32];
                         load(2 * j + h, v);
                         float y[32];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            y[k] = __uint_as_float(v[k]);
-                        }
-                        if (a.bias != nullptr) {
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) {
-                                y[k] += bias_sh[g][64 * j + 32 * h + k];
-                            }
-                        }
-                        row_grad(y, c0, limit, lab, lse2, dl, dead);
+                        row_grad(v, y, c0, limit, grad,
+                                 a.bias != nullptr ? &bias_sh[g][64 * j + 32 * h] : nullptr);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             *reinterpret_cast<uint4*>(dst + (((4 * h + q) ^ (r & 7)) << 4)) =

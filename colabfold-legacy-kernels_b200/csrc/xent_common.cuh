@@ -2,6 +2,8 @@
 // of few classes.
 #pragma once
 
+#include <climits>
+
 #include "sm100.cuh"
 
 namespace cflk {
@@ -78,23 +80,61 @@ __device__ __forceinline__ void row_stats(float (&y)[32], int c0, int V, int lab
     m = m1;
 }
 
-// 32 logits to g = dl (softmax - onehot) with the row's log2-domain lse; zeros past V and in a dead row
-__device__ __forceinline__ void row_grad(float (&y)[32], int c0, int V, int label, float lse2,
-                                         float dl, bool dead) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        y[j] = ex2(fmaf(y[j], kLog2e, -lse2));
+// What a row needs to turn logits into g = dl (softmax - onehot): its log2-domain lse, dl and
+// label (relative to the columns). A row without a token or with no class left is set so that its g
+// comes out as zeros.
+struct GradRow {
+    float lse2, dl;
+    int label;
+    __device__ __forceinline__ void kill() {
+        lse2 = kInf;
+        dl = 0.f;
+        label = INT_MIN / 2;
     }
-    const int at = label - c0;
+};
+
+// 32 accumulators of a row, columns c0.. of V, to g; `bias` (or null) is their 32 biases in shared
+// memory. Columns past V give zeros. Pairs of columns share an instruction where they can.
+__device__ __forceinline__ void row_grad(const uint32_t (&v)[32], float (&y)[32], int c0, int V,
+                                         const GradRow& row, const float* bias) {
+    const uint64_t log2e = pk2(kLog2e, kLog2e), ref = pk2(-row.lse2, -row.lse2);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        uint64_t l0 = pk2(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]));
+        uint64_t l1 = pk2(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3]));
+        if (bias != nullptr) {
+            const float4 b = reinterpret_cast<const float4*>(bias)[q];
+            l0 = add2(l0, pk2(b.x, b.y));
+            l1 = add2(l1, pk2(b.z, b.w));
+        }
+        const float2 e0 = upk2(fma2(l0, log2e, ref)), e1 = upk2(fma2(l1, log2e, ref));
+        y[4 * q] = ex2(e0.x);
+        y[4 * q + 1] = ex2(e0.y);
+        y[4 * q + 2] = ex2(e1.x);
+        y[4 * q + 3] = ex2(e1.y);
+    }
+    const int at = row.label - c0;
     if (at >= 0 && at < 32) {
+        const unsigned bit = 1u << at;
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-            y[j] -= j == at ? 1.f : 0.f;
+            if (bit & (1u << j)) {
+                y[j] -= 1.f;
+            }
         }
     }
+    const uint64_t dl = pk2(row.dl, row.dl);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        y[j] = dead || c0 + j >= V ? 0.f : y[j] * dl;
+    for (int q = 0; q < 16; ++q) {
+        const float2 g = upk2(mul2(pk2(y[2 * q], y[2 * q + 1]), dl));
+        y[2 * q] = g.x;
+        y[2 * q + 1] = g.y;
+    }
+    if (c0 + 32 > V) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            y[j] = c0 + j < V ? y[j] : 0.f;
+        }
     }
 }
 

@@ -8,13 +8,15 @@
 //
 //   * a persistent CTA an SM; it lists its labelled tokens in shared memory (blocks of 128 tokens
 //     in turn over the CTAs) and works through them 128 at a time, so positions without a label
-//     cost nothing but dx's zeros, which a warp sends as bulk copies;
+//     cost nothing but dx's zeros, which a warp sends as bulk copies. Where at least half of the
+//     tokens carry a label it takes whole blocks as tiles instead, x and dx as TMA boxes;
 //   * w stays in shared memory in one layout that serves as the K-major B of the logits and the
-//     N-major B of dx; a tile of x, gathered row by row by four warps' asynchronous copies, is the K-major A of the logits, then the N-major B of dw, then the staging of dx, whose rows
-//     leave in whole lines; g is the K-major A of dx and the M-major A of dw;
+//     N-major B of dx; a tile of x, gathered row by row by four warps' asynchronous copies, is the
+//     K-major A of the logits, then the N-major B of dw; g is the K-major A of dx and the M-major
+//     A of dw;
 //   * two warpgroups take the tiles in turn, each with its own tensor-memory slot, so one's
-//     exponentials overlap the other's products and stores; one warp issues all MMAs in a fixed
-//     order;
+//     exponentials overlap the other's products and stores; each has a warp that issues its
+//     MMAs, and dw's are issued in the order of the tiles;
 //   * each CTA leaves a float32 dw (and dbias), a second kernel adds them in order: the same bits
 //     every run.
 //
@@ -41,9 +43,10 @@ namespace {
 
 __device__ unsigned g_status;
 
-// two warpgroups of workers, then the zeroing, the MMA and four loading warps
-constexpr int kThreads = 448;
-constexpr int kZeroWarp = 8, kMmaWarp = 9, kLoad0 = 10, kLoaders = 4;
+// two warpgroups of workers, then the zeroing warp, an MMA warp for each and four loading warps
+constexpr int kThreads = 480;
+constexpr int kZeroWarp = 8, kMmaWarp = 9, kLoad0 = 11, kLoaders = 4;
+constexpr int kFwdSlots = 4;  // of logits in tensor memory
 constexpr int kRoundBlocks = 32;      // blocks of 128 tokens a CTA lists at a time
 constexpr int kRound = kRoundBlocks * 128;
 constexpr int kAtom = 128 * 128;      // 128 rows of 64 16-bit columns, 128-byte swizzle
@@ -92,6 +95,7 @@ struct HeadArgs {
     float* dw_part;      // [CTA][V][C]
     float* db_part;      // [CTA][V]
     int T, V, C;
+    bool wide;           // dx rows in 32-byte accesses
     Layout l;
 };
 
@@ -104,6 +108,20 @@ __device__ __forceinline__ void copy_wait_all() {
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
+// 32 bytes to a 32-byte boundary in one access
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::
+                     "l"(map),
+                 "r"(src), "r"(c0), "r"(c1)
+                 : "memory");
+}
+
 // `bytes` (a multiple of 16) from shared to global memory, both 16-byte aligned
 __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
@@ -111,33 +129,21 @@ __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t byt
                  : "memory");
 }
 
-// whether the phase with the given parity is complete
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 template <typename T, typename L, bool BWD>
 __global__ void __launch_bounds__(kThreads, 1)
-    head_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ HeadArgs a) {
+    head_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
+                const __grid_constant__ CUtensorMap tdx, const __grid_constant__ HeadArgs a) {
     using E = Elem<T>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t w_full, x_full[4], x_free[4], l_full[2], g_full[2], d_full[2], d_free[2],
-        drain;
+    __shared__ uint64_t w_full, x_full[4], x_free[4], dx_ready[4], l_full[kFwdSlots], d_free[kFwdSlots],
+        g_full[2], g_free[2], d_full[2], dw_done[2], drain;
     __shared__ uint32_t tmem_sh;
     __shared__ int abort_flag;
-    __shared__ float bias_sh[128];
+    __shared__ __align__(16) float bias_sh[128];
     __shared__ __align__(16) uint4 zero_sh[32];
-    __shared__ int block_count[kRoundBlocks + 1];
+    __shared__ int block_count[kRoundBlocks + 1], block_list[kRoundBlocks], dense_sh, blocks_sh;
     __shared__ float max_sh[kThreads / 32];
 
     const Layout& l = a.l;
@@ -150,6 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int vn = (a.V + 15) & ~15;   // logits columns, and K of dx
     const int cn = (a.C + 15) & ~15;   // dw columns
     const int nch = (a.C + 127) / 128; // dx goes through the slot 128 columns at a time
+    const int nmask = l.nx - 1, nshift = l.nx == 4 ? 2 : 1;  // tile g: buffer g & nmask
     const int blocks = (int)(((long long)a.T + 127) / 128);
     const int rounds = (blocks + kRoundBlocks * (int)gridDim.x - 1) / (kRoundBlocks * (int)gridDim.x);
     // token j of this CTA's block i of round rd
@@ -162,15 +169,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&w_full, 1);
             for (int i = 0; i < 4; ++i) {
                 mbar_init(&x_full[i], 32 * kLoaders / l.nx);  // the loading warps' lanes
-                mbar_init(&x_free[i], BWD ? 128 : 1);
+                mbar_init(&x_free[i], 1);
+                // a worker warp arrives once
+                mbar_init(&dx_ready[i], 4);
+            }
+            for (int i = 0; i < kFwdSlots; ++i) {
+                mbar_init(&l_full[i], 1);
+                mbar_init(&d_free[i], 4);
             }
             for (int i = 0; i < 2; ++i) {
-                mbar_init(&l_full[i], 1);
-                mbar_init(&g_full[i], 128);
+                mbar_init(&g_full[i], 4);
+                mbar_init(&g_free[i], 1);
                 mbar_init(&d_full[i], 1);
-                mbar_init(&d_free[i], 128);
+                mbar_init(&dw_done[i], 1);
             }
-            mbar_init(&drain, 1);
+            mbar_init(&drain, 2);
             abort_flag = 0;
             fence_mbar_init();
         }
@@ -227,8 +240,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     int base = 0;             // tiles of earlier rounds
-    int df = 0;               // workers: dx chunks seen
-    int freed[2] = {0, 0};    // MMA: slots drained
+    int df = 0;               // dx chunks seen (workers) or drained (MMA)
+    int stored = 0;           // loading warps: tiles of dx stored
     float db[4] = {0.f, 0.f, 0.f, 0.f};
     bool ok = true, w_ready = false;
     for (int rd = 0; rd < rounds; ++rd) {
@@ -262,8 +275,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
             block_count[lane] = x - n;
+            // the blocks with a labelled token, and whether at least half of the tokens are labelled
+            const unsigned some = __ballot_sync(0xffffffffu, n > 0);
+            if (n > 0) {
+                block_list[__popc(some & ((1u << lane) - 1))] = lane;
+            }
+            const long long left = a.T - token(rd, lane, 0);
+            const int in = warp_sum((int)min(128ll, max(0ll, left)));
             if (lane == 31) {
                 block_count[32] = x;
+                blocks_sh = __popc(some);
+                dense_sh = 2 * x >= in;
             }
         }
         __syncthreads();
@@ -295,12 +317,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncthreads();
         const int count = block_count[kRoundBlocks];
-        const int n = (count + 127) / 128;
+        // Dense rounds take whole blocks of tokens as tiles, x and dx as TMA boxes, and rows without a
+        // label as rows without a gradient; the others gather the labelled rows
+        const bool dense = dense_sh != 0;
+        const int n = dense ? blocks_sh : (count + 127) / 128;
 
+        const auto arrive_warp = [&](uint64_t* bar) {
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(bar);
+            }
+        };
         if (warp >= kLoad0) {
-            // the labelled rows of x, 16 bytes a copy, 8, 16 or 32 lanes a row; the last tile's
-            // missing rows repeat the last token (their g is zero). Each tile buffer has its
-            // own one or two warps, so as many tiles are under way as there are buffers.
+            // Each tile buffer has its own one or two warps, so as many tiles are under way as
+            // there are buffers. Gathered rows: 16 bytes a copy, 8, 16 or 32 lanes a row; the last
+            // tile's missing rows repeat the last token (their g is zero).
             const int wpt = kLoaders / l.nx, b = (warp - kLoad0) / wpt;  // warps a tile, buffer
             const int part = (warp - kLoad0) % wpt, rows = 128 / wpt;
             const int lpr = cn <= 64 ? 8 : cn <= 128 ? 16 : 32, rpw = 32 / lpr;
@@ -309,11 +340,48 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t bytes = piece * 8 < a.C ? 16 : 0;  // zeros up to the K step
             const T* x = static_cast<const T*>(a.x) + (bytes ? piece * 8 : 0);
             const uint32_t dst = smem_u32(xs + b * xbytes) + (piece >> 3) * kAtom;
+            int staged = -1;  // dense backward: the tile whose dx this buffer will hold
+            const auto store_dx = [&] {
+                ok = mbar_wait(&dx_ready[b], stored & 1, &g_status, kStatusSyncWait, &abort_flag);
+                ++stored;
+                const int t0 = (int)token(rd, block_list[staged], 0);
+                for (int i = 0; i < l.atoms; ++i) {
+                    tma_store_2d(&tdx, smem_u32(xs + b * xbytes + i * kAtom), 64 * i, t0);
+                }
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            };
             // tiles g = base + c with g % nx == b
-            for (int c = (b - base % l.nx + l.nx) % l.nx; c < n; c += l.nx) {
+            for (int c = (b - base) & nmask; c < n; c += l.nx) {
                 const int g = base + c;
+                if (dense) {
+                    if (lane == 0) {
+                        if (staged >= 0) {
+                            store_dx();
+                        } else {
+                            ok = g < l.nx || mbar_wait(&x_free[b], ((g >> nshift) - 1) & 1, &g_status,
+                                                       kStatusSyncWait, &abort_flag);
+                        }
+                    }
+                    ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                    if (!ok) {
+                        break;
+                    }
+                    // (every lane arrives: the barrier counts those of the gathering form)
+                    if (lane == 0 && part == 0) {
+                        staged = BWD ? c : -1;
+                        const int t0 = (int)token(rd, block_list[c], 0);
+                        mbar_arrive_expect_tx(&x_full[b], xbytes);
+                        for (int i = 0; i < l.atoms; ++i) {
+                            tma_load_2d(xs + b * xbytes + i * kAtom, &tx, &x_full[b], 64 * i, t0);
+                        }
+                    } else {
+                        mbar_arrive(&x_full[b]);
+                    }
+                    continue;
+                }
                 if (lane == 0) {
-                    ok = g < l.nx || mbar_wait(&x_free[b], (g / l.nx - 1) & 1, &g_status,
+                    ok = g < l.nx || mbar_wait(&x_free[b], ((g >> nshift) - 1) & 1, &g_status,
                                                kStatusSyncWait, &abort_flag);
                 }
                 ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -339,146 +407,182 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fence_async_smem();
                 mbar_arrive(&x_full[b]);
             }
-        } else if (warp == kMmaWarp && lane == 0) {
-            const uint32_t sw = smem_u32(smem);
+            if (staged >= 0 && ok) {
+                store_dx();
+            }
+            __syncwarp();
+        } else if (warp >= kMmaWarp && lane == 0) {
+            // Descriptors are made once: a step along an operand is an addition to its address field
+            // (16-byte units). K-major: a K step of 16 columns is 32 bytes, 64 columns an atom;
+            // MN-major: a K step of 16 rows is 2 KB.
             const uint32_t id_l = idesc_f16(E::kBf16, 128, vn, false, false);
             const auto k_major = [](uint32_t at) { return smem_desc(at, 16, 1024, kSwizzle128B); };
-            const auto logits = [&](int c) {
-                const int g = base + c, b = g % l.nx;
+            const uint64_t w_k = k_major(smem_u32(smem));
+            const uint64_t w_n = smem_desc(smem_u32(smem), l.vp * 128, 1024, kSwizzle128B);
+            const uint64_t x_k0 = k_major(smem_u32(xs)), g_k0 = k_major(smem_u32(gs));
+            [[maybe_unused]] const uint64_t x_n0 = smem_desc(smem_u32(xs), kAtom, 1024, kSwizzle128B);
+            [[maybe_unused]] const uint64_t g_m0 = smem_desc(smem_u32(gs), kAtom, 1024, kSwizzle128B);
+            const uint32_t w_atom = l.vp * 8, x_tile = xbytes >> 4, g_tile = gbytes >> 4;
+            constexpr uint32_t kAtom16 = kAtom >> 4;
+            // K-major A (atoms kAtom apart) times B, ksteps steps of K; b_step and b_atom: B's
+            // advance a step and an atom
+            const auto product = [&](uint32_t d, uint64_t da, uint64_t dbp, uint32_t b_step,
+                                     uint32_t b_atom, uint32_t id, int ksteps) {
+                uint32_t on = 0;
+                for (int k = 0; k < ksteps; k += 4) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        if (k + u < ksteps) {
+                            mma_ss(d, da + 2 * u, dbp + u * b_step, id, on);
+                            on = 1;
+                        }
+                    }
+                    da += kAtom16;
+                    dbp += b_atom;
+                }
+            };
+            const auto logits = [&](int c, int slot) {
+                const int g = base + c, b = g & nmask;
                 if (!w_ready) {
                     ok = ok && mbar_wait(&w_full, 0, &g_status, kStatusTmaWait, &abort_flag);
                     w_ready = true;
                 }
-                ok = ok && mbar_wait(&x_full[b], (g / l.nx) & 1, &g_status, kStatusTmaWait,
+                ok = ok && mbar_wait(&x_full[b], (g >> nshift) & 1, &g_status, kStatusTmaWait,
                                      &abort_flag);
                 if (!ok) {
                     return;
                 }
                 tc_fence_after();
-                const uint32_t sx = smem_u32(xs + b * xbytes);
-                for (int ks = 0; ks < cn / 16; ++ks) {
-                    mma_ss(tmem + 128 * (g & 1), k_major(sx + (ks >> 2) * kAtom + 32 * (ks & 3)),
-                           k_major(sw + (ks >> 2) * l.vp * 128 + 32 * (ks & 3)), id_l, ks > 0);
-                }
+                product(tmem + 128 * slot, x_k0 + b * x_tile, w_k, 2, w_atom, id_l, cn >> 4);
                 if constexpr (!BWD) {
                     mma_commit(&x_free[b]);
                 }
-                mma_commit(&l_full[g & 1]);
+                mma_commit(&l_full[slot]);
+            };
+            const auto wait = [&](uint64_t* bar, int parity) {
+                ok = ok && mbar_wait(bar, parity & 1, &g_status, kStatusSyncWait, &abort_flag);
+                tc_fence_after();
             };
             if constexpr (!BWD) {
-                for (int c = 0; ok && c < n; ++c) {
-                    const int g = base + c;
-                    if (g >= 2) {
-                        ok = mbar_wait(&d_free[g & 1], ((g >> 1) - 1) & 1, &g_status,
-                                       kStatusSyncWait, &abort_flag);
-                        tc_fence_after();
-                    }
-                    if (ok) {
-                        logits(c);
+                if (warp == kMmaWarp) {
+                    for (int c = 0; ok && c < n; ++c) {
+                        const int g = base + c;
+                        if (g >= kFwdSlots) {
+                            wait(&d_free[g % kFwdSlots], g / kFwdSlots - 1);
+                        }
+                        logits(c, g % kFwdSlots);
                     }
                 }
             } else {
-                // dx's columns [128 ch, ...) of tile c into its slot
-                const auto dx_chunk = [&](int c, int ch) {
-                    const int g = base + c, cols = min(128, cn - 128 * ch);
-                    const uint32_t id = idesc_f16(E::kBf16, 128, cols, false, true);
-                    const uint32_t sg = smem_u32(gs + (g & 1) * gbytes);
-                    for (int ks = 0; ks < vn / 16; ++ks) {
-                        mma_ss(tmem + 128 * (g & 1),
-                               k_major(sg + (ks >> 2) * kAtom + 32 * (ks & 3)),
-                               smem_desc(sw + 2 * ch * l.vp * 128 + ks * 2048, l.vp * 128, 1024,
-                                         kSwizzle128B),
-                               id, ks > 0);
-                    }
-                };
+                // This warp's tiles are those of worker group h: the logits, dx's first 128 columns
+                // and dw once g is written, dx's other columns as the slot is drained. The two
+                // warps add to dw in turn, so that its sum is always the same one.
+                const int h = warp - kMmaWarp;
                 const uint32_t id_w = idesc_f16(E::kBf16, l.vp, cn, true, true);
-                // Each warpgroup's tile goes through: logits (x has come) -> dx's first columns and
-                // dw (g is written; tiles in order, so dw's sum is always the same one) -> dx's
-                // other columns (the slot is drained) -> the tile after next. Whatever is ready
-                // is issued.
-                int tile[2] = {base & 1, 1 - (base & 1)}, stage[2] = {0, 0}, next_dw = 0;
-                unsigned long long t0 = globaltimer();
-                while (tile[0] < n || tile[1] < n) {
-                    bool moved = false;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int c = tile[h], g = base + c;
-                        if (c >= n) {
-                            continue;
-                        }
-                        if (stage[h] == 0) {
-                            if (mbar_test(&x_full[g % l.nx], (g / l.nx) & 1)) {
-                                logits(c);
-                                stage[h] = 1;
-                                moved = true;
-                            }
-                        } else if (stage[h] == 1) {
-                            if (next_dw == c && mbar_test(&g_full[h], (g >> 1) & 1)) {
-                                tc_fence_after();
-                                dx_chunk(c, 0);
-                                const uint32_t sg = smem_u32(gs + h * gbytes);
-                                const uint32_t sx = smem_u32(xs + (g % l.nx) * xbytes);
-                                for (int ks = 0; ks < 8; ++ks) {
-                                    mma_ss(dw_col,
-                                           smem_desc(sg + ks * 2048, kAtom, 1024, kSwizzle128B),
-                                           smem_desc(sx + ks * 2048, kAtom, 1024, kSwizzle128B),
-                                           id_w, g > 0 || ks > 0);
-                                }
-                                mma_commit(&d_full[h]);  // also: x's and g's reads are done
-                                ++next_dw;
-                                stage[h] = 2;
-                                moved = true;
-                            }
-                        } else if (mbar_test(&d_free[h], freed[h] & 1)) {
-                            ++freed[h];
-                            tc_fence_after();
-                            const int ch = stage[h] - 1;
-                            if (ch < nch) {
-                                dx_chunk(c, ch);
-                                mma_commit(&d_full[h]);
-                                ++stage[h];
-                            } else {
-                                tile[h] += 2;
-                                stage[h] = 0;
-                            }
-                            moved = true;
+                for (int c = (base + h) & 1; ok && c < n; c += 2) {
+                    const int g = base + c;
+                    const auto dx_chunk = [&](int ch) {
+                        product(tmem + 128 * h, g_k0 + h * g_tile, w_n + 2 * ch * w_atom, 128, 512,
+                                idesc_f16(E::kBf16, 128, min(128, cn - 128 * ch), false, true),
+                                vn >> 4);
+                        mma_commit(&d_full[h]);
+                    };
+                    logits(c, h);
+                    wait(&g_full[h], g >> 1);
+                    if (!ok) {
+                        break;
+                    }
+                    dx_chunk(0);
+                    if (g > 0) {
+                        wait(&dw_done[h ^ 1], (g - 1) >> 1);
+                        if (!ok) {
+                            break;
                         }
                     }
-                    if (moved) {
-                        t0 = globaltimer();
-                    } else if (!ok || *(volatile int*)&abort_flag ||
-                               globaltimer() - t0 > kWaitLimitNs) {
-                        atomicOr(&g_status, kStatusSyncWait);
-                        abort_flag = 1;
-                        break;
+                    const uint64_t dg = g_m0 + h * g_tile, dx = x_n0 + (g & nmask) * x_tile;
+#pragma unroll 2
+                    for (int ks = 0; ks < 8; ++ks) {
+                        mma_ss(dw_col, dg + 128 * ks, dx + 128 * ks, id_w, g > 0 || ks > 0);
+                    }
+                    mma_commit(&x_free[g & nmask]);
+                    mma_commit(&dw_done[h]);
+                    for (int ch = 1; ok && ch <= nch; ++ch) {
+                        wait(&d_free[h], df++);
+                        if (ok && ch < nch) {
+                            dx_chunk(ch);
+                        }
                     }
                 }
             }
         } else if (BWD && warp == kZeroWarp) {
             // zeros for the rows without a label: a bulk copy of a zeroed row each
-            for (int i = lane; i < kRound - count; i += 32) {
-                const int t = list[kRound - 1 - i];
+            // (dense: of the blocks without one)
+            for (int i = lane; i < (dense ? kRound : kRound - count); i += 32) {
+                const int blk = i >> 7;
+                long long t = list[kRound - 1 - i];
+                if (dense) {
+                    t = token(rd, blk, i & 127);
+                    t = t < a.T && block_count[blk + 1] == block_count[blk] ? t : -1;
+                }
                 if (t >= 0) {
-                    bulk_store(static_cast<T*>(a.dx) + (long long)t * a.C, smem_u32(zero_sh),
+                    bulk_store(static_cast<T*>(a.dx) + t * a.C, smem_u32(zero_sh),
                                a.C * 2);
                 }
             }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            // then dbias: the columns 2 lane, 2 lane + 1 of each 64 of g, tile by tile
+            for (int c = 0; a.bias != nullptr && c < n; ++c) {
+                const int g = base + c, h = g & 1;
+                mbar_wait(&g_full[h], (g >> 1) & 1, &g_status, kStatusSyncWait, &abort_flag);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    if (q * 64 >= vn) {
+                        break;
+                    }
+                    const uint8_t* p = gs + h * gbytes + q * kAtom + (lane & 3) * 4;
+                    float s0[2] = {0.f, 0.f}, s1[2] = {0.f, 0.f};
+#pragma unroll 16
+                    for (int row = 0; row < 128; ++row) {
+                        const float2 w = E::unpack(*reinterpret_cast<const uint32_t*>(
+                            p + row * 128 + (((lane >> 2) ^ (row & 7)) << 4)));
+                        s0[row & 1] += w.x;
+                        s1[row & 1] += w.y;
+                    }
+                    db[2 * q] += s0[0] + s0[1];
+                    db[2 * q + 1] += s1[0] + s1[1];
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&g_free[h]);
+                }
+            }
         } else if (warp < kZeroWarp) {
             const int h = warp >> 2;                       // warpgroup
             const int r = ((warp & 3) << 5) | lane;        // row of the tile, tensor-memory lane
-            const uint32_t slot = tmem + 128 * h + tmem_lane_base(warp);
             for (int c = (base + h) & 1; c < n; c += 2) {
-                const int g = base + c, b = g % l.nx;
-                const bool live = c * 128 + r < count;
-                const int tok = list[min(c * 128 + r, count - 1)];
+                const int g = base + c;
+                const int sl = BWD ? h : g % kFwdSlots, turn = BWD ? g >> 1 : g / kFwdSlots;
+                const uint32_t slot = tmem + 128 * sl + tmem_lane_base(warp);
+                const long long at = dense ? token(rd, block_list[c], r)
+                                           : (long long)list[min(c * 128 + r, count - 1)];
+                const long long tok = min(at, (long long)a.T - 1);
                 const int lab = label_of(labels, tok, a.V);
-                [[maybe_unused]] float lse2 = 0.f, dl = 0.f;
+                const bool live = dense ? lab >= 0 && at < a.T : c * 128 + r < count;
+                [[maybe_unused]] GradRow grad;
                 if constexpr (BWD) {
-                    lse2 = a.lse_in[tok];
-                    dl = a.dloss[tok] * scale;
+                    grad.lse2 = live ? a.lse_in[tok] : -kInf;
+                    grad.dl = live ? a.dloss[tok] * scale : 0.f;
+                    grad.label = lab;
+                    if (grad.lse2 == -kInf) {
+                        grad.kill();
+                    }
+                    if (a.bias != nullptr && g >= 2) {
+                        // dbias has been summed from this warpgroup's last g
+                        mbar_wait(&g_free[h], ((g >> 1) - 1) & 1, &g_status, kStatusSyncWait,
+                                  &abort_flag);
+                    }
                 }
-                mbar_wait(&l_full[h], (g >> 1) & 1, &g_status, kStatusMmaWait, &abort_flag);
+                mbar_wait(&l_full[sl], turn & 1, &g_status, kStatusMmaWait, &abort_flag);
                 tc_fence_after();
                 if constexpr (!BWD) {
                     float m = -kInf, s = 0.f, at_label = 0.f;
@@ -494,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         row_stats(y, c0, a.V, lab, m, s, at_label);
                     }
                     tc_fence_before();
-                    mbar_arrive(&d_free[h]);
+                    arrive_warp(&d_free[sl]);
                     if (live) {
                         const bool none = m == -kInf && s == 0.f;
                         const float l2 = log2f(s);
@@ -502,18 +606,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                         a.loss[tok] = none ? 0.f : kLn2 * (m + l2) - at_label;
                     }
                 } else {
-                    const bool dead = !live || lse2 == -kInf;
                     uint8_t* grow = gs + h * gbytes + r * 128;
+                    const int b = g & nmask;
+                    uint8_t* xrow = xs + b * xbytes + r * 128;
                     for (int c0 = 0; c0 < vn; c0 += 32) {
                         uint32_t v[32];
                         tmem_ld32(slot + c0, v);
                         tmem_wait_ld();
-                        float y[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            y[j] = __uint_as_float(v[j]) + bias_sh[c0 + j];
+                        if (dense && !live && c0 == 0 && !isfinite(__uint_as_float(v[0]))) {
+                            // a row without a label may hold anything, and dw multiplies it by
+                            // zeros: NaN and infinities (which every logit shows) are cleared
+                            for (int p = 0; p < 8 * l.atoms; ++p) {
+                                *reinterpret_cast<uint4*>(
+                                    xrow + (p >> 3) * kAtom + (((p & 7) ^ (r & 7)) << 4)) =
+                                    make_uint4(0, 0, 0, 0);
+                            }
                         }
-                        row_grad(y, c0, a.V, lab, lse2, dl, dead);
+                        float y[32];
+                        row_grad(v, y, c0, a.V, grad, a.bias != nullptr ? bias_sh + c0 : nullptr);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             *reinterpret_cast<uint4*>(
@@ -527,71 +637,70 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     fence_async_smem();
                     tc_fence_before();
-                    mbar_arrive(&g_full[h]);
-                    if (a.bias != nullptr) {
-                        // columns 2 lane, 2 lane + 1 of each atom over this warp's 32 rows
-                        named_sync(1 + h, 128);
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            if (q * 64 >= vn) {
-                                break;
-                            }
-                            const uint8_t* p = gs + h * gbytes + q * kAtom;
-#pragma unroll 8
-                            for (int i = 0; i < 32; ++i) {
-                                const int row = 32 * (warp & 3) + i;
-                                const float2 w = E::unpack(*reinterpret_cast<const uint32_t*>(
-                                    p + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) +
-                                    (lane & 3) * 4));
-                                db[2 * q] += w.x;
-                                db[2 * q + 1] += w.y;
-                            }
-                        }
-                    }
-                    // dx into the tile of x, which its products no longer read
-                    uint8_t* xrow = xs + b * xbytes + r * 128;
+                    arrive_warp(&g_full[h]);
+                    // dx. Dense: into the tile of x, which its products no longer read, for the loading
+                    // warp to store. Gathered: a thread stores its row, whole 32-byte sectors where
+                    // the rows allow it
+                    T* out = static_cast<T*>(a.dx) + (long long)tok * a.C;
                     for (int ch = 0; ch < nch; ++ch) {
                         mbar_wait(&d_full[h], df & 1, &g_status, kStatusMmaWait, &abort_flag);
                         ++df;
+                        if (ch == 0) {
+                            // dw has read g and x
+                            mbar_wait(&dw_done[h], (g >> 1) & 1, &g_status, kStatusMmaWait,
+                                      &abort_flag);
+                        }
                         tc_fence_after();
                         const int end = min(128, a.C - 128 * ch);
                         for (int c0 = 0; c0 < end; c0 += 32) {
                             uint32_t v[32];
                             tmem_ld32(slot + c0, v);
                             tmem_wait_ld();
-                            const int col = 128 * ch + c0;
+                            if (c0 + 32 >= end) {
+                                tc_fence_before();
+                                arrive_warp(&d_free[h]);
+                            }
+                            uint32_t o[16];
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                uint32_t o[4];
+                            for (int i = 0; i < 16; ++i) {
+                                o[i] = E::pack(__uint_as_float(v[2 * i]) * inv,
+                                               __uint_as_float(v[2 * i + 1]) * inv);
+                            }
+                            T* p = out + 128 * ch + c0;
+                            if (dense) {
+                                const int col = 128 * ch + c0;
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    o[i] = E::pack(__uint_as_float(v[8 * q + 2 * i]) * inv,
-                                                   __uint_as_float(v[8 * q + 2 * i + 1]) * inv);
+                                for (int q = 0; q < 4; ++q) {
+                                    *reinterpret_cast<uint4*>(
+                                        xrow + (col >> 6) * kAtom +
+                                        (((((col >> 3) & 4) + q) ^ (r & 7)) << 4)) =
+                                        live ? make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2],
+                                                          o[4 * q + 3])
+                                             : make_uint4(0, 0, 0, 0);
                                 }
-                                *reinterpret_cast<uint4*>(
-                                    xrow + (col >> 6) * kAtom +
-                                    (((((col >> 3) & 4) + q) ^ (r & 7)) << 4)) =
-                                    make_uint4(o[0], o[1], o[2], o[3]);
+                            } else if (live && a.wide) {
+#pragma unroll
+                                for (int q = 0; q < 2; ++q) {
+                                    if (c0 + 16 * q < end) {
+                                        store32(p + 16 * q, &o[8 * q]);
+                                    }
+                                }
+                            } else if (live) {
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    if (c0 + 8 * q < end) {
+                                        *reinterpret_cast<uint4*>(p + 8 * q) =
+                                            make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2],
+                                                       o[4 * q + 3]);
+                                    }
+                                }
                             }
                         }
-                        tc_fence_before();
-                        mbar_arrive(&d_free[h]);
                     }
-                    named_sync(1 + h, 128);
-                    // whole rows out: 8, 16 or 32 lanes a row of up to 64, 128 or 256 columns
-                    const int lpr = a.C <= 64 ? 8 : a.C <= 128 ? 16 : 32;
-                    const int piece = lane & (lpr - 1), sub = lane / lpr, rpw = 32 / lpr;
-                    for (int i = (warp & 3) * rpw + sub; i < 128; i += 4 * rpw) {
-                        if (c * 128 + i < count && piece * 8 < a.C) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(
-                                xs + b * xbytes + (piece >> 3) * kAtom + i * 128 +
-                                (((piece & 7) ^ (i & 7)) << 4));
-                            reinterpret_cast<uint4*>(static_cast<T*>(a.dx) +
-                                                     (long long)list[c * 128 + i] * a.C)[piece] = w;
-                        }
+                    if (dense) {
+                        fence_async_smem();
+                        arrive_warp(&dx_ready[b]);
                     }
-                    fence_async_smem();
-                    mbar_arrive(&x_free[b]);
                 }
             }
         }
@@ -603,10 +712,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kZeroWarp && lane == 0) {
         mbar_wait(&w_full, 0, &g_status, kStatusTmaWait, nullptr, kDrainLimitNs);
     }
-    if (BWD && warp == kZeroWarp) {
+    if (BWD && warp >= kZeroWarp) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
-    if (warp == kMmaWarp && lane == 0) {
+    if ((warp == kMmaWarp || warp == kMmaWarp + 1) && lane == 0) {
         mma_commit(&drain);
         mbar_wait(&drain, 0, &g_status, kStatusMmaWait, nullptr, kDrainLimitNs);
     }
@@ -615,7 +724,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     if constexpr (BWD) {
-        float* db_sh = reinterpret_cast<float*>(list);  // [warp of the workers][128]
         if (warp < kZeroWarp) {
             const int h = warp >> 2, w = warp & 3;
             // dw: lane = class; with 64 rows lanes 32 w + i (i < 16) hold class 16 w + i
@@ -645,21 +753,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            if (a.bias != nullptr) {
+        } else if (warp == kZeroWarp && a.bias != nullptr) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    db_sh[(4 * h + w) * 128 + 64 * (q >> 1) + 2 * lane + (q & 1)] = db[q];
+            for (int q = 0; q < 4; ++q) {
+                const int v = 64 * (q >> 1) + 2 * lane + (q & 1);
+                if (v < a.V) {
+                    a.db_part[(long long)blockIdx.x * a.V + v] = db[q] * inv;
                 }
             }
-        }
-        __syncthreads();
-        if (a.bias != nullptr && (int)threadIdx.x < a.V) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s += db_sh[i * 128 + threadIdx.x];
-            }
-            a.db_part[(long long)blockIdx.x * a.V + threadIdx.x] = s * inv;
         }
         tc_fence_before();
     }
@@ -730,7 +831,8 @@ int head_grid(int64_t T) {
 }
 
 template <typename T, typename L, bool BWD>
-cudaError_t launch(const HeadCall& c, const CUtensorMap& tw, const HeadArgs& a) {
+cudaError_t launch(const HeadCall& c, const CUtensorMap& tx, const CUtensorMap& tw,
+                   const CUtensorMap& tdx, const HeadArgs& a) {
     auto kern = head_kernel<T, L, BWD>;
     static bool done[kMaxDevices] = {};
     int dev = 0;
@@ -747,7 +849,7 @@ cudaError_t launch(const HeadCall& c, const CUtensorMap& tw, const HeadArgs& a) 
             done[dev] = true;
         }
     }
-    kern<<<head_grid(c.T), kThreads, a.l.bytes, c.stream>>>(tw, a);
+    kern<<<head_grid(c.T), kThreads, a.l.bytes, c.stream>>>(tx, tw, tdx, a);
     return cudaGetLastError();
 }
 
@@ -776,26 +878,33 @@ cudaError_t xent_head(const HeadCall& c, bool bwd, bool& map_ok) {
     a.T = (int)c.T;
     a.V = (int)c.V;
     a.C = (int)c.C;
+    a.wide = c.C % 16 == 0 && reinterpret_cast<uintptr_t>(c.dx) % 32 == 0;
     const int grid = head_grid(c.T);
     a.dw_part = static_cast<float*>(c.workspace);
     a.db_part = a.dw_part + (size_t)grid * c.V * c.C;
     const CUtensorMapDataType t =
         c.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    CUtensorMap tw;
-    const uint64_t dw[2] = {(uint64_t)c.C, (uint64_t)c.V}, st[1] = {(uint64_t)c.C};
-    const uint32_t bw[2] = {64, (uint32_t)a.l.vp};
-    map_ok = encode_tiled(&tw, t, 2, 2, c.w, dw, st, bw, CU_TENSOR_MAP_SWIZZLE_128B);
+    CUtensorMap tx, tw, tdx;
+    const uint64_t dims[2] = {(uint64_t)c.C, (uint64_t)c.T}, dw[2] = {(uint64_t)c.C, (uint64_t)c.V};
+    const uint64_t st[1] = {(uint64_t)c.C};
+    const uint32_t box[2] = {64, 128}, bw[2] = {64, (uint32_t)a.l.vp};
+    map_ok = encode_tiled(&tx, t, 2, 2, c.x, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B) &&
+             encode_tiled(&tw, t, 2, 2, c.w, dw, st, bw, CU_TENSOR_MAP_SWIZZLE_128B);
+    tdx = tx;
+    if (map_ok && bwd) {
+        map_ok = encode_tiled(&tdx, t, 2, 2, c.dx, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
     if (!map_ok) {
         return cudaSuccess;
     }
     const auto run = [&](auto tag) -> cudaError_t {
         using T = decltype(tag);
         if (!bwd) {
-            return c.labels_64 ? launch<T, long long, false>(c, tw, a)
-                               : launch<T, int, false>(c, tw, a);
+            return c.labels_64 ? launch<T, long long, false>(c, tx, tw, tdx, a)
+                               : launch<T, int, false>(c, tx, tw, tdx, a);
         }
-        cudaError_t e = c.labels_64 ? launch<T, long long, true>(c, tw, a)
-                                    : launch<T, int, true>(c, tw, a);
+        cudaError_t e = c.labels_64 ? launch<T, long long, true>(c, tx, tw, tdx, a)
+                                    : launch<T, int, true>(c, tx, tw, tdx, a);
         if (e == cudaSuccess) {
             const int blocks = (a.V * a.C / 4 + 31) / 32 + (c.bias != nullptr ? (a.V + 31) / 32 : 0);
             head_reduce_kernel<T><<<blocks, 256, 0, c.stream>>>(
