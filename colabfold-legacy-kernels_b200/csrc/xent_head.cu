@@ -43,14 +43,15 @@ namespace {
 
 __device__ unsigned g_status;
 
-// two warpgroups of workers, then the zeroing warp, an MMA warp for each and four loading warps
-constexpr int kThreads = 480;
-constexpr int kZeroWarp = 8, kMmaWarp = 9, kLoad0 = 11, kLoaders = 4;
+// two warpgroups of workers, then, a warp for each of them, the column sums of g (dbias), the MMAs;
+// and four loading warps
+constexpr int kThreads = 512;
+constexpr int kSumWarp = 8, kMmaWarp = 10, kLoad0 = 12, kLoaders = 4;
 constexpr int kFwdSlots = 4;  // of logits in tensor memory
 constexpr int kRoundBlocks = 32;      // blocks of 128 tokens a CTA lists at a time
 constexpr int kRound = kRoundBlocks * 128;
 constexpr int kAtom = 128 * 128;      // 128 rows of 64 16-bit columns, 128-byte swizzle
-constexpr int kDynamicMax = 227 * 1024 - 2048;  // beside the static shared memory
+constexpr int kDynamicMax = 227 * 1024 - 3072;  // beside the static shared memory
 constexpr int kSms = 148;
 constexpr unsigned long long kDrainLimitNs = 200000000ull;
 
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ __align__(16) float bias_sh[128];
     __shared__ __align__(16) uint4 zero_sh[32];
     __shared__ int block_count[kRoundBlocks + 1], block_list[kRoundBlocks], dense_sh, blocks_sh;
-    __shared__ float max_sh[kThreads / 32];
+    __shared__ float max_sh[kThreads / 32], db_sh[2][128];
 
     const Layout& l = a.l;
     const L* labels = static_cast<const L*>(a.labels);
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_alloc(&tmem_sh, 512);
         tmem_relinquish();
     }
-    if (warp == kZeroWarp) {
+    if (warp == kSumWarp) {
         zero_sh[lane] = make_uint4(0, 0, 0, 0);
         fence_async_smem();
     }
@@ -230,9 +231,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_sh;
-    const uint32_t dw_col = tmem + 256;
+    // Tensor memory: two slots of 128 columns for dx and 256 columns for dw; where dw takes at most
+    // 128 and the logits at most 64, the logits have columns of their own and run a tile ahead,
+    // else they share the slot with dx.
+    const bool ahead = BWD && cn <= 128 && l.vp == 64;
+    const uint32_t dw_col = tmem + (ahead ? 384 : 256);
+    const auto logits_col = [&](int slot) {
+        return tmem + (ahead ? 256 + 64 * slot : 128 * slot);
+    };
 
-    if (warp == kZeroWarp && lane == 0) {
+    if (warp == kSumWarp && lane == 0) {
         mbar_arrive_expect_tx(&w_full, l.atoms * l.vp * 128);
         for (int i = 0; i < l.atoms; ++i) {
             tma_load_2d(smem + i * l.vp * 128, &tw, &w_full, 64 * i, 0);
@@ -244,6 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stored = 0;           // loading warps: tiles of dx stored
     float db[4] = {0.f, 0.f, 0.f, 0.f};
     bool ok = true, w_ready = false;
+#pragma unroll 1
     for (int rd = 0; rd < rounds; ++rd) {
         // list this round's tokens: the labelled ones in order from the front, the others from
         // the back
@@ -345,6 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = mbar_wait(&dx_ready[b], stored & 1, &g_status, kStatusSyncWait, &abort_flag);
                 ++stored;
                 const int t0 = (int)token(rd, block_list[staged], 0);
+#pragma unroll 1
                 for (int i = 0; i < l.atoms; ++i) {
                     tma_store_2d(&tdx, smem_u32(xs + b * xbytes + i * kAtom), 64 * i, t0);
                 }
@@ -352,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             };
             // tiles g = base + c with g % nx == b
+#pragma unroll 1
             for (int c = (b - base) & nmask; c < n; c += l.nx) {
                 const int g = base + c;
                 if (dense) {
@@ -372,6 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         staged = BWD ? c : -1;
                         const int t0 = (int)token(rd, block_list[c], 0);
                         mbar_arrive_expect_tx(&x_full[b], xbytes);
+#pragma unroll 1
                         for (int i = 0; i < l.atoms; ++i) {
                             tma_load_2d(xs + b * xbytes + i * kAtom, &tx, &x_full[b], 64 * i, t0);
                         }
@@ -425,20 +437,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t w_atom = l.vp * 8, x_tile = xbytes >> 4, g_tile = gbytes >> 4;
             constexpr uint32_t kAtom16 = kAtom >> 4;
             // K-major A (atoms kAtom apart) times B, ksteps steps of K; b_step and b_atom: B's
-            // advance a step and an atom
+            // advance a step, and over the fourth. Loops of one MMA stay in the instruction cache
+            // that the workers' long code sweeps (unrolled by four: 1500 cycles where this takes X)
             const auto product = [&](uint32_t d, uint64_t da, uint64_t dbp, uint32_t b_step,
                                      uint32_t b_atom, uint32_t id, int ksteps) {
-                uint32_t on = 0;
-                for (int k = 0; k < ksteps; k += 4) {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        if (k + u < ksteps) {
-                            mma_ss(d, da + 2 * u, dbp + u * b_step, id, on);
-                            on = 1;
-                        }
-                    }
-                    da += kAtom16;
-                    dbp += b_atom;
+#pragma unroll 1
+                for (int k = 0; k < ksteps; ++k) {
+                    mma_ss(d, da, dbp, id, k);
+                    const bool last = (k & 3) == 3;
+                    da += last ? kAtom16 - 6 : 2;
+                    dbp += last ? b_atom : b_step;
                 }
             };
             const auto logits = [&](int c, int slot) {
@@ -453,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return;
                 }
                 tc_fence_after();
-                product(tmem + 128 * slot, x_k0 + b * x_tile, w_k, 2, w_atom, id_l, cn >> 4);
+                product(logits_col(slot), x_k0 + b * x_tile, w_k, 2, w_atom - 6, id_l, cn >> 4);
                 if constexpr (!BWD) {
                     mma_commit(&x_free[b]);
                 }
@@ -479,16 +487,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // warps add to dw in turn, so that its sum is always the same one.
                 const int h = warp - kMmaWarp;
                 const uint32_t id_w = idesc_f16(E::kBf16, l.vp, cn, true, true);
+#pragma unroll 1
                 for (int c = (base + h) & 1; ok && c < n; c += 2) {
                     const int g = base + c;
                     const auto dx_chunk = [&](int ch) {
-                        product(tmem + 128 * h, g_k0 + h * g_tile, w_n + 2 * ch * w_atom, 128, 512,
+                        product(tmem + 128 * h, g_k0 + h * g_tile, w_n + 2 * ch * w_atom, 128, 128,
                                 idesc_f16(E::kBf16, 128, min(128, cn - 128 * ch), false, true),
                                 vn >> 4);
                         mma_commit(&d_full[h]);
                     };
-                    logits(c, h);
+                    if (!ahead || c < 2) {
+                        logits(c, h);
+                    }
                     wait(&g_full[h], g >> 1);
+                    if (ahead && c >= 2) {
+                        wait(&d_free[h], df++);
+                    }
                     if (!ok) {
                         break;
                     }
@@ -500,12 +514,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     const uint64_t dg = g_m0 + h * g_tile, dx = x_n0 + (g & nmask) * x_tile;
-#pragma unroll 2
+#pragma unroll 1
                     for (int ks = 0; ks < 8; ++ks) {
                         mma_ss(dw_col, dg + 128 * ks, dx + 128 * ks, id_w, g > 0 || ks > 0);
                     }
                     mma_commit(&x_free[g & nmask]);
                     mma_commit(&dw_done[h]);
+                    if (ahead) {
+                        if (c + 2 < n) {
+                            logits(c + 2, h);
+                        } else {
+                            wait(&d_free[h], df++);
+                        }
+                        continue;
+                    }
+#pragma unroll 1
                     for (int ch = 1; ok && ch <= nch; ++ch) {
                         wait(&d_free[h], df++);
                         if (ok && ch < nch) {
@@ -514,10 +537,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-        } else if (BWD && warp == kZeroWarp) {
+        } else if (BWD && (warp == kSumWarp || warp == kSumWarp + 1)) {
             // zeros for the rows without a label: a bulk copy of a zeroed row each
             // (dense: of the blocks without one)
-            for (int i = lane; i < (dense ? kRound : kRound - count); i += 32) {
+            for (int i = threadIdx.x - 32 * kSumWarp; i < (dense ? kRound : kRound - count); i += 64) {
                 const int blk = i >> 7;
                 long long t = list[kRound - 1 - i];
                 if (dense) {
@@ -531,8 +554,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             // then dbias: the columns 2 lane, 2 lane + 1 of each 64 of g, tile by tile
-            for (int c = 0; a.bias != nullptr && c < n; ++c) {
-                const int g = base + c, h = g & 1;
+            const int h = warp - kSumWarp;
+            for (int c = (base + h) & 1; a.bias != nullptr && c < n; c += 2) {
+                const int g = base + c;
                 mbar_wait(&g_full[h], (g >> 1) & 1, &g_status, kStatusSyncWait, &abort_flag);
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
@@ -541,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const uint8_t* p = gs + h * gbytes + q * kAtom + (lane & 3) * 4;
                     float s0[2] = {0.f, 0.f}, s1[2] = {0.f, 0.f};
-#pragma unroll 16
+#pragma unroll 8
                     for (int row = 0; row < 128; ++row) {
                         const float2 w = E::unpack(*reinterpret_cast<const uint32_t*>(
                             p + row * 128 + (((lane >> 2) ^ (row & 7)) << 4)));
@@ -556,13 +580,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(&g_free[h]);
                 }
             }
-        } else if (warp < kZeroWarp) {
+        } else if (warp < kSumWarp) {
             const int h = warp >> 2;                       // warpgroup
             const int r = ((warp & 3) << 5) | lane;        // row of the tile, tensor-memory lane
+#pragma unroll 1
             for (int c = (base + h) & 1; c < n; c += 2) {
                 const int g = base + c;
                 const int sl = BWD ? h : g % kFwdSlots, turn = BWD ? g >> 1 : g / kFwdSlots;
-                const uint32_t slot = tmem + 128 * sl + tmem_lane_base(warp);
+                const uint32_t slot = logits_col(sl) + tmem_lane_base(warp);
+                [[maybe_unused]] const uint32_t dx_slot = tmem + 128 * sl + tmem_lane_base(warp);
                 const long long at = dense ? token(rd, block_list[c], r)
                                            : (long long)list[min(c * 128 + r, count - 1)];
                 const long long tok = min(at, (long long)a.T - 1);
@@ -586,6 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_after();
                 if constexpr (!BWD) {
                     float m = -kInf, s = 0.f, at_label = 0.f;
+#pragma unroll 1
                     for (int c0 = 0; c0 < a.V; c0 += 32) {
                         uint32_t v[32];
                         tmem_ld32(slot + c0, v);
@@ -609,6 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint8_t* grow = gs + h * gbytes + r * 128;
                     const int b = g & nmask;
                     uint8_t* xrow = xs + b * xbytes + r * 128;
+#pragma unroll 1
                     for (int c0 = 0; c0 < vn; c0 += 32) {
                         uint32_t v[32];
                         tmem_ld32(slot + c0, v);
@@ -616,6 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (dense && !live && c0 == 0 && !isfinite(__uint_as_float(v[0]))) {
                             // a row without a label may hold anything, and dw multiplies it by
                             // zeros: NaN and infinities (which every logit shows) are cleared
+#pragma unroll 1
                             for (int p = 0; p < 8 * l.atoms; ++p) {
                                 *reinterpret_cast<uint4*>(
                                     xrow + (p >> 3) * kAtom + (((p & 7) ^ (r & 7)) << 4)) =
@@ -642,60 +671,55 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // warp to store. Gathered: a thread stores its row, whole 32-byte sectors where
                     // the rows allow it
                     T* out = static_cast<T*>(a.dx) + (long long)tok * a.C;
+#pragma unroll 1
                     for (int ch = 0; ch < nch; ++ch) {
                         mbar_wait(&d_full[h], df & 1, &g_status, kStatusMmaWait, &abort_flag);
                         ++df;
+                        tc_fence_after();
+                        const int end = min(128, a.C - 128 * ch);
                         if (ch == 0) {
                             // dw has read g and x
                             mbar_wait(&dw_done[h], (g >> 1) & 1, &g_status, kStatusMmaWait,
                                       &abort_flag);
                         }
-                        tc_fence_after();
-                        const int end = min(128, a.C - 128 * ch);
+#pragma unroll 1
                         for (int c0 = 0; c0 < end; c0 += 32) {
-                            uint32_t v[32];
-                            tmem_ld32(slot + c0, v);
+                            uint32_t v[32], o[16];
+                            tmem_ld32(dx_slot + c0, v);
                             tmem_wait_ld();
-                            if (c0 + 32 >= end) {
-                                tc_fence_before();
-                                arrive_warp(&d_free[h]);
-                            }
-                            uint32_t o[16];
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
                                 o[i] = E::pack(__uint_as_float(v[2 * i]) * inv,
                                                __uint_as_float(v[2 * i + 1]) * inv);
                             }
-                            T* p = out + 128 * ch + c0;
+                            const int col = 128 * ch + c0;
                             if (dense) {
-                                const int col = 128 * ch + c0;
+                                uint8_t* p = xrow + (col >> 6) * kAtom;
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) {
                                     *reinterpret_cast<uint4*>(
-                                        xrow + (col >> 6) * kAtom +
-                                        (((((col >> 3) & 4) + q) ^ (r & 7)) << 4)) =
+                                        p + (((((col >> 3) & 4) + q) ^ (r & 7)) << 4)) =
                                         live ? make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2],
                                                           o[4 * q + 3])
                                              : make_uint4(0, 0, 0, 0);
                                 }
-                            } else if (live && a.wide) {
-#pragma unroll
-                                for (int q = 0; q < 2; ++q) {
-                                    if (c0 + 16 * q < end) {
-                                        store32(p + 16 * q, &o[8 * q]);
-                                    }
-                                }
                             } else if (live) {
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) {
-                                    if (c0 + 8 * q < end) {
-                                        *reinterpret_cast<uint4*>(p + 8 * q) =
-                                            make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2],
-                                                       o[4 * q + 3]);
+                                    if (c0 + 8 * q >= end) {
+                                        break;
+                                    }
+                                    if (!a.wide) {
+                                        *reinterpret_cast<uint4*>(out + col + 8 * q) = make_uint4(
+                                            o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+                                    } else if (q % 2 == 0) {
+                                        store32(out + col + 8 * q, &o[4 * q]);
                                     }
                                 }
                             }
                         }
+                        tc_fence_before();
+                        arrive_warp(&d_free[h]);
                     }
                     if (dense) {
                         fence_async_smem();
@@ -709,10 +733,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
     }
     // every copy has landed and every MMA is done before shared and tensor memory go
-    if (warp == kZeroWarp && lane == 0) {
+    if (warp == kSumWarp && lane == 0) {
         mbar_wait(&w_full, 0, &g_status, kStatusTmaWait, nullptr, kDrainLimitNs);
     }
-    if (BWD && warp >= kZeroWarp) {
+    if (BWD && warp >= kSumWarp) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     if ((warp == kMmaWarp || warp == kMmaWarp + 1) && lane == 0) {
@@ -724,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     if constexpr (BWD) {
-        if (warp < kZeroWarp) {
+        if (warp < kSumWarp) {
             const int h = warp >> 2, w = warp & 3;
             // dw: lane = class; with 64 rows lanes 32 w + i (i < 16) hold class 16 w + i
             const int v = l.vp == 128 ? 32 * w + lane : 16 * w + lane;
@@ -753,14 +777,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-        } else if (warp == kZeroWarp && a.bias != nullptr) {
+        } else if (warp < kMmaWarp && a.bias != nullptr) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int v = 64 * (q >> 1) + 2 * lane + (q & 1);
-                if (v < a.V) {
-                    a.db_part[(long long)blockIdx.x * a.V + v] = db[q] * inv;
-                }
+                db_sh[warp - kSumWarp][64 * (q >> 1) + 2 * lane + (q & 1)] = db[q];
             }
+        }
+        __syncthreads();
+        if (a.bias != nullptr && (int)threadIdx.x < a.V) {
+            a.db_part[(long long)blockIdx.x * a.V + threadIdx.x] =
+                (db_sh[0][threadIdx.x] + db_sh[1][threadIdx.x]) * inv;
         }
         tc_fence_before();
     }
