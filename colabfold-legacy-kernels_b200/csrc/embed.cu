@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "capi_internal.h"
 #include "cflk_b200.h"
@@ -49,7 +50,7 @@ __global__ void __launch_bounds__(kFwdThreads)
         for (int u = 0; u < kFwdUnroll; ++u) {
             r[u] = row;
             c[u] = col;
-            id[u] = row < T ? (long long)ids[row] : -1;
+            id[u] = (long long)ids[min(row, T - 1)];
             row += drow;
             col += dcol;
             if (col >= cv) {
@@ -57,13 +58,16 @@ __global__ void __launch_bounds__(kFwdThreads)
                 ++row;
             }
         }
+        // no branch round a load: an id outside the table reads its row 0 and drops it
         float v[kFwdUnroll][VEC];
 #pragma unroll
         for (int u = 0; u < kFwdUnroll; ++u) {
             const bool ok = id[u] >= 0 && id[u] < V;
-            if (ok) {
-                load_vec<TI, VEC>(table + (id[u] * cv + c[u]) * VEC, v[u]);
-            }
+            load_vec<TI, VEC>(table + ((ok ? id[u] : 0) * cv + c[u]) * VEC, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kFwdUnroll; ++u) {
+            const bool ok = id[u] >= 0 && id[u] < V;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 v[u][i] = ok ? v[u][i] * scale : 0.f;
@@ -105,6 +109,7 @@ cudaError_t launch_embed(cudaStream_t s, const void* ids, const void* table, voi
 constexpr int kSortThreads = 256, kSortWarps = kSortThreads / 32, kSortRounds = 4;
 constexpr int kSortItems = kSortThreads * kSortRounds;  // a block's consecutive pairs
 constexpr int kMaxDigit = 9;                            // bits of a pass
+constexpr int kFewBlocks = 32;                          // no scan kernel up to these
 
 // An id outside [0, V) sorts as V, behind every row.
 template <typename Id>
@@ -166,7 +171,8 @@ __global__ void __launch_bounds__(kSortThreads)
     }
 }
 
-// Each block puts its pairs at their places. Warp w owns the block's pairs [w 32 kSortRounds,
+// Each block puts its pairs at their places. Where the blocks are few (scanned 0) it adds the counts
+// of a digit itself, else it takes their prefix from sort_scan_kernel. Warp w owns the block's pairs [w 32 kSortRounds,
 // (w + 1) 32 kSortRounds) in rounds of 32: a pair's rank among the warp's of its digit is the
 // digit's running count plus the lower lanes of the round with the same digit, so equal digits
 // keep their order. FIRST: the pairs are (ids[t], t).
@@ -174,7 +180,8 @@ template <typename Key, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads)
     sort_scatter_kernel(const Key* __restrict__ keys, const int* __restrict__ toks, int T,
                         unsigned V, int shift, int bits, const int* __restrict__ counts,
-                        const int* __restrict__ totals, int nblocks, unsigned* __restrict__ okeys,
+                        const int* __restrict__ totals, int nblocks, int scanned,
+                        unsigned* __restrict__ okeys,
                         int* __restrict__ otoks) {
     __shared__ int run[kSortWarps][1 << kMaxDigit];
     __shared__ int base[1 << kMaxDigit];
@@ -188,7 +195,26 @@ __global__ void __launch_bounds__(kSortThreads)
     }
     // exclusive prefix of the totals: two digits a thread, a scan over the warps
     const int d0 = 2 * tid;
-    const int t0 = d0 < bins ? totals[d0] : 0, t1 = d0 + 1 < bins ? totals[d0 + 1] : 0;
+    int t[2] = {0, 0}, lower[2] = {0, 0};  // a digit's pairs in all blocks, and in those before
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        if (d0 + k >= bins) {
+            continue;
+        }
+        const int* row = counts + (long long)(d0 + k) * nblocks;
+        if (scanned) {
+            t[k] = totals[d0 + k];
+            lower[k] = row[blockIdx.x];
+        } else {
+#pragma unroll 8
+            for (int b = 0; b < nblocks; ++b) {
+                const int n = row[b];
+                t[k] += n;
+                lower[k] += b < (int)blockIdx.x ? n : 0;
+            }
+        }
+    }
+    const int t0 = t[0], t1 = t[1];
     int x = t0 + t1;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -205,10 +231,10 @@ __global__ void __launch_bounds__(kSortThreads)
         before += w < warp ? warp_sum[w] : 0;
     }
     if (d0 < bins) {
-        base[d0] = before + counts[(long long)d0 * nblocks + blockIdx.x];
+        base[d0] = before + lower[0];
     }
     if (d0 + 1 < bins) {
-        base[d0 + 1] = before + t0 + counts[(long long)(d0 + 1) * nblocks + blockIdx.x];
+        base[d0 + 1] = before + t0 + lower[1];
     }
     const long long at = (long long)blockIdx.x * kSortItems + warp * 32 * kSortRounds + lane;
     unsigned key[kSortRounds];
@@ -264,19 +290,64 @@ __global__ void __launch_bounds__(kSortThreads)
 // ------------------------------------------------------------------------------------------
 // backward: sums over the sorted list
 // ------------------------------------------------------------------------------------------
-constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32, kSumUnroll = 8;
+constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
+
+// Rows without a token get zeros: 32 rows a warp a step, each lane looks its row up in the sorted
+// keys.
+template <int VEC>
+__device__ __forceinline__ void zero_rows(const unsigned* keys, float* dtable, int n, unsigned V,
+                                          int C, long long warp, long long warps) {
+    const int lane = threadIdx.x & 31;
+    for (long long r0 = warp * 32; r0 < (long long)V; r0 += warps * 32) {
+        const long long row = r0 + lane;
+        bool empty = row < (long long)V;
+        if (empty) {
+            int lo = 0, hi = n;  // first place with keys >= row
+            while (lo < hi) {
+                const int mid = (int)(((long long)lo + hi) >> 1);
+                if (keys[mid] < (unsigned)row) {
+                    lo = mid + 1;
+                } else {
+                    hi = mid;
+                }
+            }
+            empty = lo >= n || keys[lo] != (unsigned)row;
+        }
+        unsigned todo = __ballot_sync(0xffffffffu, empty);
+        float zero[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            zero[i] = 0.f;
+        }
+        while (todo != 0) {
+            const int r = __ffs(todo) - 1;
+            todo &= todo - 1;
+            float* dst = dtable + (r0 + r) * C;
+            for (int col = lane * VEC; col < C; col += 32 * VEC) {
+                store_vec<float, VEC>(dst + col, zero);
+            }
+        }
+    }
+}
 
 // A warp sums chunk `c` of the sorted list (len pairs) over one slab of 32 VEC channels. Rows
 // whose pairs all lie in the chunk are written; the sum of a row that began before the chunk goes
-// to partial[c][0], that of a row that began in it and goes on after it to partial[c][1].
+// to partial[c][0], that of a row that began in it and goes on after it to partial[c][1]. The
+// blocks past the first sum_blocks write the rows without a token meanwhile.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSumThreads)
     embed_sum_kernel(const unsigned* __restrict__ keys, const int* __restrict__ toks,
                      const T* __restrict__ dout, float* __restrict__ dtable,
                      float* __restrict__ partial, int n, unsigned V, int C, int slabs, int chunks,
-                     int len, float scale) {
+                     int len, int sum_blocks, float scale) {
+    constexpr int kUnroll = 8;
     const int lane = threadIdx.x & 31;
     const long long item = (long long)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
+    if ((int)blockIdx.x >= sum_blocks) {
+        zero_rows<VEC == 1 ? 1 : 4>(keys, dtable, n, V, C, item - (long long)sum_blocks * kSumWarps,
+                       (long long)(gridDim.x - sum_blocks) * kSumWarps);
+        return;
+    }
     if (item >= (long long)chunks * slabs) {
         return;
     }
@@ -286,6 +357,7 @@ __global__ void __launch_bounds__(kSumThreads)
     const int p0 = c * len, p1 = min(p0 + len, n);
     const unsigned prev = p0 > 0 ? keys[p0 - 1] : 0xffffffffu;
     const unsigned next = p1 < n ? keys[p1] : 0xffffffffu;
+    const T* src = dout + (on ? col : 0);
     float acc[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -308,21 +380,22 @@ __global__ void __launch_bounds__(kSumThreads)
             store_vec<float, VEC>(dst, o);
         }
     };
-    for (int p = p0; p < p1; p += kSumUnroll) {
-        unsigned k[kSumUnroll];
-        float v[kSumUnroll][VEC];
+    for (int p = p0; p < p1; p += kUnroll) {
+        unsigned k[kUnroll];
+        int t[kUnroll];
+        float v[kUnroll][VEC];
+        // (no branch round a load: what is past the chunk or outside the table is dropped below)
 #pragma unroll
-        for (int u = 0; u < kSumUnroll; ++u) {
-            k[u] = p + u < p1 ? keys[p + u] : V;
+        for (int u = 0; u < kUnroll; ++u) {
+            k[u] = keys[min(p + u, p1 - 1)];
+            t[u] = toks[min(p + u, p1 - 1)];
         }
 #pragma unroll
-        for (int u = 0; u < kSumUnroll; ++u) {
-            if (k[u] < V && on) {
-                load_vec<T, VEC>(dout + (long long)toks[p + u] * C + col, v[u]);
-            }
+        for (int u = 0; u < kUnroll; ++u) {
+            load_vec<T, VEC>(src + (long long)t[u] * C, v[u]);
         }
 #pragma unroll
-        for (int u = 0; u < kSumUnroll; ++u) {
+        for (int u = 0; u < kUnroll; ++u) {
             if (p + u < p1) {
                 if (k[u] != cur) {
                     flush(false);
@@ -399,54 +472,268 @@ __device__ __forceinline__ void join_row(const unsigned* keys, float* dtable,
     store_vec<float, VEC>(dtable + (long long)row * C + col, acc);
 }
 
-// The rows that cross chunks (the first chunks * slabs warps) and, by every warp, the rows
-// without a token: 32 rows a step, each lane looks its row up in the sorted keys.
 template <int VEC>
 __global__ void __launch_bounds__(kSumThreads)
-    embed_finish_kernel(const unsigned* __restrict__ keys, float* __restrict__ dtable,
-                        const float* __restrict__ partial, int n, unsigned V, int C, int slabs,
-                        int chunks, int len, float scale) {
-    const int lane = threadIdx.x & 31;
-    const long long warp = (long long)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
-    const long long warps = (long long)gridDim.x * kSumWarps;
-    for (long long item = warp; item < (long long)chunks * slabs; item += warps) {
+    embed_join_kernel(const unsigned* __restrict__ keys, float* __restrict__ dtable,
+                      const float* __restrict__ partial, int n, unsigned V, int C, int slabs,
+                      int chunks, int len, float scale) {
+    const long long item = (long long)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
+    if (item < (long long)chunks * slabs) {
         const int c = (int)(item / slabs);
         join_row<VEC>(keys, dtable, partial, n, V, C, c, (int)(item - (long long)c * slabs), len,
                       scale);
     }
-    for (long long r0 = warp * 32; r0 < (long long)V; r0 += warps * 32) {
-        const long long row = r0 + lane;
-        bool empty = row < (long long)V;
-        if (empty) {
-            int lo = 0, hi = n;  // first place with keys >= row
-            while (lo < hi) {
-                const int mid = (int)(((long long)lo + hi) >> 1);
-                if (keys[mid] < (unsigned)row) {
-                    lo = mid + 1;
+}
+
+// ------------------------------------------------------------------------------------------
+// backward of a small table: sorted CTA by CTA
+// ------------------------------------------------------------------------------------------
+// Where the table's slab of 4 GL channels fits shared memory, a CTA sorts its own tokens there, up to
+// kLocalTokens at a time: a counting sort by row whose ranks keep the tokens' order. Groups of GL
+// lanes then take equal ranges of the sorted list, each row's sum in registers, so the only
+// traffic is dout's; rows that end inside a range go to the table, those at its ends to a list
+// whose runs of one row are added in order. The CTAs' tables are added in order by
+// embed_local_reduce_kernel.
+constexpr int kLocalThreads = 1024, kLocalWarps = kLocalThreads / 32;
+constexpr int kLocalTokens = 4096, kLocalRounds = kLocalTokens / kLocalThreads;
+constexpr int kLocalSmem = 200 * 1024;
+
+struct LocalSmem {
+    int table, ends, end_row, base, count, key, tok, bytes;
+};
+__host__ __device__ inline LocalSmem local_smem(int V, int lanes) {
+    LocalSmem m;
+    int at = 0;
+    const auto take = [&](int n) {
+        const int o = at;
+        at += (n + 15) / 16 * 16;
+        return o;
+    };
+    m.table = take(V * lanes * 16);
+    m.ends = take(kLocalThreads * 2 * 16);
+    m.end_row = take(kLocalThreads / lanes * 2 * 4);
+    m.base = take((V + 1) * 4);
+    m.count = take(kLocalWarps * V * 2);
+    m.key = take(kLocalTokens * 2);
+    m.tok = take(kLocalTokens * 2);
+    m.bytes = at;
+    return m;
+}
+
+template <typename T, typename Id, int GL>
+__global__ void __launch_bounds__(kLocalThreads, 1)
+    embed_local_kernel(const Id* __restrict__ ids, const T* __restrict__ dout,
+                       float* __restrict__ partial, long long n, int V, int C, long long per) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int kGroups = kLocalThreads / GL, kUnroll = 8;
+    const LocalSmem m = local_smem(V, GL);
+    float4* table = reinterpret_cast<float4*>(smem + m.table);
+    float4* ends = reinterpret_cast<float4*>(smem + m.ends);
+    int* end_row = reinterpret_cast<int*>(smem + m.end_row);
+    int* base = reinterpret_cast<int*>(smem + m.base);
+    uint16_t* count = reinterpret_cast<uint16_t*>(smem + m.count);
+    uint16_t* skey = reinterpret_cast<uint16_t*>(smem + m.key);
+    uint16_t* stok = reinterpret_cast<uint16_t*>(smem + m.tok);
+    __shared__ int warp_total[kLocalWarps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int group = tid / GL, gl = tid % GL;
+    const int col = (blockIdx.y * GL + gl) * 4;
+    const bool on = col < C;
+    for (int i = tid; i < V * GL; i += kLocalThreads) {
+        table[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const long long t_end = min(n, (blockIdx.x + 1) * per);
+    for (long long t0 = blockIdx.x * per; t0 < t_end; t0 += kLocalTokens) {
+        // ranks among the warp's tokens of the same row
+        for (int i = tid; i < kLocalWarps * V; i += kLocalThreads) {
+            count[i] = 0;
+        }
+        int key[kLocalRounds], rank[kLocalRounds];
+#pragma unroll
+        for (int r = 0; r < kLocalRounds; ++r) {
+            const long long t = t0 + warp * (32 * kLocalRounds) + 32 * r + lane;
+            const long long id = t < t_end ? (long long)ids[t] : -1;
+            key[r] = id >= 0 && id < V ? (int)id : -1;
+        }
+        __syncthreads();
+        uint16_t* mine = count + warp * V;
+#pragma unroll
+        for (int r = 0; r < kLocalRounds; ++r) {
+            const unsigned same = __match_any_sync(0xffffffffu, key[r]);
+            const int before = __popc(same & ((1u << lane) - 1));
+            rank[r] = key[r] >= 0 ? mine[key[r]] + before : 0;
+            __syncwarp();
+            if (key[r] >= 0 && lane == 31 - __clz(same)) {
+                mine[key[r]] = (uint16_t)(rank[r] + 1);
+            }
+            __syncwarp();
+        }
+        __syncthreads();
+        // a thread a row: the warps' first places; then the rows' (V at most kLocalThreads)
+        int total = 0;
+        if (tid < V) {
+#pragma unroll 8
+            for (int w = 0; w < kLocalWarps; ++w) {
+                const int c = count[w * V + tid];
+                count[w * V + tid] = (uint16_t)total;
+                total += c;
+            }
+        }
+        int x = total;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, d);
+            x += lane >= d ? y : 0;
+        }
+        if (lane == 31) {
+            warp_total[warp] = x;
+        }
+        __syncthreads();
+        int lower = x - total, listed = 0;
+#pragma unroll
+        for (int w = 0; w < kLocalWarps; ++w) {
+            lower += w < warp ? warp_total[w] : 0;
+            listed += warp_total[w];
+        }
+        if (tid < V) {
+            base[tid] = lower;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kLocalRounds; ++r) {
+            if (key[r] >= 0) {
+                const int at = base[key[r]] + mine[key[r]] + rank[r];
+                skey[at] = (uint16_t)key[r];
+                stok[at] = (uint16_t)(warp * (32 * kLocalRounds) + 32 * r + lane);
+            }
+        }
+        __syncthreads();
+        // sums of this group's range
+        const int len = (listed + kGroups - 1) / kGroups;
+        const int p0 = group * len, p1 = min(listed, p0 + len);
+        if (gl == 0) {
+            end_row[2 * group] = -1;
+            end_row[2 * group + 1] = -1;
+        }
+        if (p0 < p1) {
+            const T* src = dout + t0 * C + (on ? col : 0);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            int cur = skey[p0];
+            bool first = true;
+            const auto flush = [&](bool last) {
+                if (first || last) {
+                    const int e = 2 * group + (first ? 0 : 1);
+                    ends[e * GL + gl] = acc;
+                    if (gl == 0) {
+                        end_row[e] = cur;
+                    }
                 } else {
-                    hi = mid;
+                    float4 a = table[cur * GL + gl];
+                    a.x += acc.x;
+                    a.y += acc.y;
+                    a.z += acc.z;
+                    a.w += acc.w;
+                    table[cur * GL + gl] = a;
+                }
+            };
+            for (int p = p0; p < p1; p += kUnroll) {
+                Raw<T, 4> v[kUnroll];
+                int k[kUnroll];
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    const int q = min(p + u, p1 - 1);
+                    k[u] = skey[q];
+                    v[u] = load_raw<T, 4>(src + (long long)stok[q] * C);
+                }
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    if (p + u < p1) {
+                        if (k[u] != cur) {
+                            flush(false);
+                            first = false;
+                            cur = k[u];
+                            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+                        float y[4];
+                        unpack_raw<T, 4>(v[u], y);
+                        acc.x += y[0];
+                        acc.y += y[1];
+                        acc.z += y[2];
+                        acc.w += y[3];
+                    }
                 }
             }
-            empty = lo >= n || keys[lo] != (unsigned)row;
+            flush(true);
         }
-        unsigned todo = __ballot_sync(0xffffffffu, empty);
-        float zero[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            zero[i] = 0.f;
-        }
-        while (todo != 0) {
-            const int r = __ffs(todo) - 1;
-            todo &= todo - 1;
-            float* dst = dtable + (r0 + r) * C;
-            for (int col = lane * VEC; col < C; col += 32 * VEC) {
-                store_vec<float, VEC>(dst + col, zero);
+        __syncthreads();
+        // the ranges' ends, sorted by row: the first entry of a row adds them up
+        for (int e = group; e < 2 * kGroups; e += kGroups) {
+            const int row = end_row[e];
+            int prev = -1;
+            for (int q = e - 1; q >= 0 && prev < 0; --q) {
+                prev = end_row[q];
             }
+            if (row < 0 || prev == row) {
+                continue;
+            }
+            float4 a = table[row * GL + gl];
+            for (int q = e; q < 2 * kGroups && (end_row[q] == row || end_row[q] < 0); ++q) {
+                if (end_row[q] == row) {
+                    const float4 b = ends[q * GL + gl];
+                    a.x += b.x;
+                    a.y += b.y;
+                    a.z += b.z;
+                    a.w += b.w;
+                }
+            }
+            table[row * GL + gl] = a;
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    if (on) {
+        for (int row = group; row < V; row += kGroups) {
+            *reinterpret_cast<float4*>(partial + ((long long)blockIdx.x * V + row) * C + col) =
+                table[row * GL + gl];
         }
     }
 }
 
+// The CTAs' sums in order: four channels a thread, eight threads over the CTAs.
+__global__ void __launch_bounds__(256)
+    embed_local_reduce_kernel(const float4* __restrict__ partial, int parts, int total4,
+                              float scale, float4* __restrict__ dtable) {
+    __shared__ float4 sh[8][32];
+    const int r = threadIdx.x & 31, seg = threadIdx.x >> 5, i = blockIdx.x * 32 + r;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < total4) {
+#pragma unroll 8
+        for (int p = seg; p < parts; p += 8) {
+            const float4 v = partial[(long long)p * total4 + i];
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+        }
+    }
+    sh[seg][r] = s;
+    __syncthreads();
+    if (seg == 0 && i < total4) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) {
+            s.x += sh[k][r].x;
+            s.y += sh[k][r].y;
+            s.z += sh[k][r].z;
+            s.w += sh[k][r].w;
+        }
+        dtable[i] = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
+    }
+}
+
 struct BwdPlan {
+    bool local;
+    int lanes, parts;  // local: lanes of a token, CTAs a slab
+    long long per;     // tokens a CTA
     int passes, bits, nblocks;
     int slabs, chunks, len, vec;
     size_t off_counts, off_totals, off_keys[2], off_toks[2], off_partial, bytes;
@@ -457,10 +744,22 @@ size_t round256(size_t n) {
 }
 
 // Everything the backward does follows from T, V, C and the channel vector. False: too large.
-bool plan_bwd(int64_t T, int64_t V, int64_t C, bool vec, BwdPlan& p) {
+bool plan_bwd(int64_t T, int64_t V, int64_t C, int vec, BwdPlan& p) {
     if (T >= (int64_t(1) << 31) - kSortItems || V >= (int64_t(1) << 31) - 1 ||
         C >= (int64_t(1) << 31)) {
         return false;
+    }
+    p.lanes = C <= 32 ? 8 : C <= 64 ? 16 : 32;
+    p.local = vec >= 4 && V <= kLocalThreads && local_smem((int)V, p.lanes).bytes <= kLocalSmem;
+    if (p.local) {
+        p.slabs = (int)((C + 4 * p.lanes - 1) / (4 * p.lanes));
+        // a CTA an SM, of at least 512 tokens
+        const int64_t want = std::max<int64_t>(1, kSms / p.slabs);
+        p.per = std::max<int64_t>(512, (T + want - 1) / want);
+        p.parts = (int)((T + p.per - 1) / p.per);
+        p.off_partial = 0;
+        p.bytes = round256((size_t)p.parts * V * C * 4);
+        return true;
     }
     int width = 1;
     while ((int64_t(1) << width) <= V) {
@@ -469,11 +768,11 @@ bool plan_bwd(int64_t T, int64_t V, int64_t C, bool vec, BwdPlan& p) {
     p.passes = (width + kMaxDigit - 1) / kMaxDigit;
     p.bits = (width + p.passes - 1) / p.passes;
     p.nblocks = (int)((T + kSortItems - 1) / kSortItems);
-    p.vec = vec ? 4 : 1;
+    p.vec = vec;
     p.slabs = (int)((C + 32 * p.vec - 1) / (32 * p.vec));
-    // chunks: enough warps to fill the machine (16 a SM), at least 8 pairs each
-    const int64_t want = std::max<int64_t>(1, 16 * kSms / p.slabs);
-    p.len = (int)std::max<int64_t>(8, (T + want - 1) / want);
+    // chunks: enough warps to fill the machine (48 a SM), of at least 16 pairs
+    const int64_t want = std::max<int64_t>(1, 48 * kSms / p.slabs);
+    p.len = (int)std::max<int64_t>(16, (T + want - 1) / want);
     p.chunks = (int)((T + p.len - 1) / p.len);
     size_t at = 0;
     const auto take = [&](size_t n) {
@@ -492,10 +791,46 @@ bool plan_bwd(int64_t T, int64_t V, int64_t C, bool vec, BwdPlan& p) {
     return true;
 }
 
+template <typename T, typename Id, int GL>
+cudaError_t launch_embed_local(cudaStream_t s, const void* ids, const void* dout, float* dtable,
+                               int64_t n, int64_t V, int64_t C, float scale, float* partial,
+                               const BwdPlan& p) {
+    auto kern = embed_local_kernel<T, Id, GL>;
+    static bool done[kMaxDevices] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= kMaxDevices || !done[dev])) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLocalSmem);
+        if (e == cudaSuccess && dev < kMaxDevices) {
+            done[dev] = true;
+        }
+    }
+    if (e != cudaSuccess) {
+        return e;
+    }
+    kern<<<dim3(p.parts, p.slabs), kLocalThreads, local_smem((int)V, GL).bytes, s>>>(
+        static_cast<const Id*>(ids), static_cast<const T*>(dout), partial, n, (int)V, (int)C,
+        p.per);
+    const int total4 = (int)(V * C / 4);
+    embed_local_reduce_kernel<<<(total4 + 31) / 32, 256, 0, s>>>(
+        reinterpret_cast<const float4*>(partial), p.parts, total4, scale,
+        reinterpret_cast<float4*>(dtable));
+    return cudaGetLastError();
+}
+
 template <typename T, typename Id>
 cudaError_t launch_embed_bwd(cudaStream_t s, const void* ids, const void* dout, float* dtable,
                              int64_t n, int64_t V, int64_t C, float scale, uint8_t* ws,
                              const BwdPlan& p) {
+    if (p.local) {
+        float* partial = reinterpret_cast<float*>(ws + p.off_partial);
+        return p.lanes == 8    ? launch_embed_local<T, Id, 8>(s, ids, dout, dtable, n, V, C, scale,
+                                                              partial, p)
+               : p.lanes == 16 ? launch_embed_local<T, Id, 16>(s, ids, dout, dtable, n, V, C,
+                                                               scale, partial, p)
+                               : launch_embed_local<T, Id, 32>(s, ids, dout, dtable, n, V, C,
+                                                               scale, partial, p);
+    }
     int* counts = reinterpret_cast<int*>(ws + p.off_counts);
     int* totals = reinterpret_cast<int*>(ws + p.off_totals);
     unsigned* keys[2];
@@ -517,37 +852,46 @@ cudaError_t launch_embed_bwd(cudaStream_t s, const void* ids, const void* dout, 
             sort_count_kernel<unsigned><<<p.nblocks, kSortThreads, 0, s>>>(
                 keys[cur], (int)n, (unsigned)V, shift, p.bits, counts, p.nblocks);
         }
-        sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(
-            counts, totals, bins, p.nblocks);
+        const int scanned = p.nblocks > kFewBlocks;
+        if (scanned) {
+            sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(
+                counts, totals, bins, p.nblocks);
+        }
         if (pass == 0) {
             sort_scatter_kernel<Id, true><<<p.nblocks, kSortThreads, 0, s>>>(
                 static_cast<const Id*>(ids), nullptr, (int)n, (unsigned)V, shift, p.bits, counts,
-                totals, p.nblocks, keys[cur], toks[cur]);
+                totals, p.nblocks, scanned, keys[cur], toks[cur]);
         } else {
             sort_scatter_kernel<unsigned, false><<<p.nblocks, kSortThreads, 0, s>>>(
                 keys[cur], toks[cur], (int)n, (unsigned)V, shift, p.bits, counts, totals,
-                p.nblocks, keys[cur ^ 1], toks[cur ^ 1]);
+                p.nblocks, scanned, keys[cur ^ 1], toks[cur ^ 1]);
             cur ^= 1;
         }
     }
     const int64_t items = (int64_t)p.chunks * p.slabs;
     const unsigned sum_grid = (unsigned)((items + kSumWarps - 1) / kSumWarps);
-    const unsigned fin_grid = (unsigned)std::min<int64_t>(
-        4 * kSms, std::max<int64_t>(sum_grid, (V + 32 * kSumWarps - 1) / (32 * kSumWarps)));
-    if (p.vec == 4) {
-        embed_sum_kernel<T, 4><<<sum_grid, kSumThreads, 0, s>>>(
+    // blocks for the rows without a token
+    const unsigned zero_grid = (unsigned)std::min<int64_t>(
+        4 * kSms, (V + 32 * kSumWarps - 1) / (32 * kSumWarps));
+    const auto sum = [&](auto tag) {
+        constexpr int VEC = decltype(tag)::value;
+        embed_sum_kernel<T, VEC><<<sum_grid + zero_grid, kSumThreads, 0, s>>>(
             keys[cur], toks[cur], static_cast<const T*>(dout), dtable, partial, (int)n,
-            (unsigned)V, (int)C, p.slabs, p.chunks, p.len, scale);
-        embed_finish_kernel<4><<<fin_grid, kSumThreads, 0, s>>>(
-            keys[cur], dtable, partial, (int)n, (unsigned)V, (int)C, p.slabs, p.chunks, p.len,
-            scale);
+            (unsigned)V, (int)C, p.slabs, p.chunks, p.len, (int)sum_grid, scale);
+        if (p.chunks > 1) {
+            embed_join_kernel<VEC><<<sum_grid, kSumThreads, 0, s>>>(
+                keys[cur], dtable, partial, (int)n, (unsigned)V, (int)C, p.slabs, p.chunks, p.len,
+                scale);
+        }
+    };
+    if (p.vec == 8) {
+        if constexpr (sizeof(T) == 2) {
+            sum(std::integral_constant<int, 8>{});
+        }
+    } else if (p.vec == 4) {
+        sum(std::integral_constant<int, 4>{});
     } else {
-        embed_sum_kernel<T, 1><<<sum_grid, kSumThreads, 0, s>>>(
-            keys[cur], toks[cur], static_cast<const T*>(dout), dtable, partial, (int)n,
-            (unsigned)V, (int)C, p.slabs, p.chunks, p.len, scale);
-        embed_finish_kernel<1><<<fin_grid, kSumThreads, 0, s>>>(
-            keys[cur], dtable, partial, (int)n, (unsigned)V, (int)C, p.slabs, p.chunks, p.len,
-            scale);
+        sum(std::integral_constant<int, 1>{});
     }
     return cudaGetLastError();
 }
@@ -594,6 +938,11 @@ extern "C" int cflk_embed(void* stream, int table_dtype, int out_dtype, int ids_
         return fail(kInvalidArgument, "embed: null buffer");
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (V == 0) {  // no row to read: zeros
+        const cudaError_t e = cudaMemsetAsync(out, 0, (size_t)T * (size_t)C * (out_dtype == kF32 ? 4 : 2), s);
+        return e == cudaSuccess ? kOk
+                                : fail(kInternal, std::string("embed: ") + cudaGetErrorString(e));
+    }
     const auto run = [&](auto ti, auto to) -> cudaError_t {
         using TI = decltype(ti);
         using TO = decltype(to);
@@ -624,11 +973,14 @@ extern "C" int cflk_embed_bwd_workspace_size(int64_t T, int64_t V, int64_t C, si
     if (T == 0 || V == 0 || C == 0) {
         return kOk;
     }
-    BwdPlan a, b;
-    if (!plan_bwd(T, V, C, false, a) || !plan_bwd(T, V, C, true, b)) {
-        return fail(kInvalidArgument, "embed_bwd: T and V must be below 2^31");
+    // whichever vector the type and the buffers' alignment take
+    for (const int vec : {1, 4, 8}) {
+        BwdPlan p;
+        if (!plan_bwd(T, V, C, vec, p)) {
+            return fail(kInvalidArgument, "embed_bwd: T and V must be below 2^31");
+        }
+        *bytes = std::max(*bytes, p.bytes);
     }
-    *bytes = std::max(a.bytes, b.bytes);  // whichever the buffers' alignment takes
     return kOk;
 }
 
@@ -659,10 +1011,14 @@ extern "C" int cflk_embed_bwd(void* stream, int dtype, int ids_64, const void* i
                    ? kOk
                    : fail(kInternal, std::string("embed_bwd: ") + cudaGetErrorString(e));
     }
-    // four channels a lane (8 or 16 bytes of dout, 16 of dtable) when the rows allow it
-    const size_t want = dtype == kF32 ? 16 : 8;
-    const bool vec = C % 4 == 0 && reinterpret_cast<uintptr_t>(dout) % want == 0 &&
-                     aligned16(dtable);
+    // eight or four channels a lane (16 bytes of dout and 32 of dtable, or half) where the rows
+    // allow it
+    const auto fits = [&](int v) {
+        const size_t bytes = (size_t)v * (dtype == kF32 ? 4 : 2);
+        return C % v == 0 && reinterpret_cast<uintptr_t>(dout) % bytes == 0 &&
+               reinterpret_cast<uintptr_t>(dtable) % (4 * v) == 0;
+    };
+    const int vec = dtype != kF32 && fits(8) ? 8 : fits(4) ? 4 : 1;
     BwdPlan p;
     if (!plan_bwd(T, V, C, vec, p)) {
         return fail(kInvalidArgument, "embed_bwd: T and V must be below 2^31");

@@ -95,13 +95,14 @@ template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
     if constexpr (VEC == 1) {
         p[0] = Elem<T>::from_f(v[0]);
+    } else if constexpr (sizeof(T) == 4 && VEC == 8) {
+        // one 32-byte access (p 32-byte aligned): two of 16 would each write half sectors
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]),
+                     "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                     : "memory");
     } else if constexpr (sizeof(T) == 4) {
-        static_assert(VEC % 4 == 0);
-#pragma unroll
-        for (int i = 0; i < VEC / 4; ++i) {
-            reinterpret_cast<float4*>(p)[i] =
-                make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        }
+        static_assert(VEC == 4);
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     } else if constexpr (VEC == 4) {
         *reinterpret_cast<uint2*>(p) =
             make_uint2(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]));
