@@ -29,6 +29,7 @@ constexpr int kBlocksPerSm = 4;    // at most 64 registers a thread: all residen
 constexpr int kBlocks = 148 * kBlocksPerSm;
 constexpr int kChunk = 16384;        // elements
 constexpr int kTable = 900;          // 32 KB of kernel parameters at most
+constexpr float kInfF = __builtin_huge_valf();
 constexpr int kUnroll = 4;           // 16-byte loads a thread keeps in flight
 
 struct Table {
@@ -82,29 +83,52 @@ __device__ __forceinline__ double block_sum(double x) {
     return s;
 }
 
-// The squares are taken and added in float64: those of float32 (and bf16) values overflow float32
-// from 2^64 on and vanish below 2^-75.
+// The sum of a vector's squares: in float32 (three roundings at most, 16-bit types' squares are
+// exact), then widened, one conversion for 4 or 8 elements: a conversion each would bound the kernel
+// (300 M bf16 elements 132 us). A sum that left float32's normal range is taken again in
+// float64: squares overflow float32 from 2^64 on and lose bits below 2^-63.
+template <typename T>
+__device__ __forceinline__ double vector_sumsq(const Raw<T, 16 / (int)sizeof(T)>& r) {
+    constexpr int V = 16 / (int)sizeof(T);
+    float y[V];
+    unpack_raw<T, V>(r, y);
+    float s = 0.f;
+    if constexpr (V == 8) {
+        const float a = fmaf(y[1], y[1], y[0] * y[0]), b = fmaf(y[3], y[3], y[2] * y[2]);
+        const float c = fmaf(y[5], y[5], y[4] * y[4]), d = fmaf(y[7], y[7], y[6] * y[6]);
+        s = (a + b) + (c + d);
+    } else {
+        s = fmaf(y[1], y[1], y[0] * y[0]) + fmaf(y[3], y[3], y[2] * y[2]);
+    }
+    if (s >= 0x1p-90f && s < kInfF) {
+        return (double)s;
+    }
+    double t = 0.0;
+#pragma unroll 1
+    for (int k = 0; k < V; ++k) {
+        float x = y[0];  // a select, not an index into local memory
+#pragma unroll
+        for (int q = 1; q < V; ++q) {
+            x = q == k ? y[q] : x;
+        }
+        t = fma((double)x, (double)x, t);
+    }
+    return t;
+}
+
 template <typename T>
 __device__ __forceinline__ double chunk_sumsq(const T* p, long long numel, int at_chunk) {
     constexpr int V = 16 / (int)sizeof(T);
-    double acc = 0.0;
-    const auto add = [&](float x) {
-        const double d = (double)x;
-        acc = fma(d, d, acc);
-    };
     const int head = head_of<T>(p, numel);
     const long long body = (numel - head) / V * V;  // whole 16-byte vectors
-    if (at_chunk == 0) {
-        // the unaligned ends, fewer than V elements each
-        const long long tail = numel - head - body;
+    // the unaligned ends, fewer than V elements each, with the first chunk
+    float end0 = 0.f, end1 = 0.f;
+    if (at_chunk == 0 && threadIdx.x < V) {
         const int i = threadIdx.x;
-        if (i < head) {
-            add(Elem<T>::to_f(p[i]));
-        }
-        if (i < tail) {
-            add(Elem<T>::to_f(p[head + body + i]));
-        }
+        end0 = i < head ? Elem<T>::to_f(p[i]) : 0.f;
+        end1 = i < numel - head - body ? Elem<T>::to_f(p[head + body + i]) : 0.f;
     }
+    double acc = 0.0;
     const T* q = p + head;
     const long long b = (long long)at_chunk * kChunk;
     const long long e = b + kChunk < body ? b + kChunk : body;
@@ -113,30 +137,34 @@ __device__ __forceinline__ double chunk_sumsq(const T* p, long long numel, int a
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const long long j = i + (long long)u * kThreads * V;
-            if (j < e) {
-                v[u] = load_raw<T, V>(q + j);
-            }
+            v[u] = load_raw<T, V>(q + (j < e ? j : i));
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             if (i + (long long)u * kThreads * V < e) {
-                float y[V];
-                unpack_raw<T, V>(v[u], y);
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    add(y[k]);
-                }
+                acc += vector_sumsq<T>(v[u]);
             }
         }
     }
-    return acc;
+    return acc + fma((double)end0, (double)end0, (double)end1 * end1);
+}
+
+// The chunks of block `b`: a contiguous range, so that a block looks its first tensor up once.
+__device__ __forceinline__ void block_range(const Table& t, int& c0, int& c1) {
+    c0 = (int)((long long)t.chunks * blockIdx.x / gridDim.x);
+    c1 = (int)((long long)t.chunks * (blockIdx.x + 1) / gridDim.x);
 }
 
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     sumsq_kernel(const __grid_constant__ Table t, double* __restrict__ partial) {
     double acc = 0.0;
-    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int i = find_tensor(t, c);
+    int c0, c1;
+    block_range(t, c0, c1);
+    int i = find_tensor(t, c0);
+    for (int c = c0; c < c1; ++c) {
+        while (i + 1 < t.n && t.first[i + 1] <= c) {
+            ++i;
+        }
         const int at = c - t.first[i];
         const int type = t.type[i] & 15;
         const void* p = t.src[i];
@@ -199,9 +227,7 @@ __device__ __forceinline__ void chunk_scale(const TI* p, TO* o, long long numel,
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 const long long j = i + (long long)u * kThreads * V;
-                if (j < e) {
-                    v[u] = load_raw<TI, V>(q + j);
-                }
+                v[u] = load_raw<TI, V>(q + (j < e ? j : i));
             }
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
@@ -236,8 +262,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out != nullptr) {
         *norm_out = norm;
     }
-    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int i = find_tensor(t, c);
+    // backwards: what the norm's kernel read last is what L2 still holds
+    int c0, c1;
+    block_range(t, c0, c1);
+    int i = c1 > c0 ? find_tensor(t, c1 - 1) : 0;
+    for (int c = c1 - 1; c >= c0; --c) {
+        while (t.first[i] > c) {
+            --i;
+        }
         const int at = c - t.first[i];
         const int ti = t.type[i] & 15, to = t.type[i] >> 4;
         const long long m = t.numel[i];
