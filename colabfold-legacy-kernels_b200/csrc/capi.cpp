@@ -31,6 +31,9 @@ __attribute__((weak)) unsigned read_and_clear_status_xent() {
 __attribute__((weak)) unsigned read_and_clear_status_head() {
     return 0;
 }
+__attribute__((weak)) unsigned read_and_clear_status_few() {
+    return 0;
+}
 
 int fail(int code, const std::string& msg) {
     t_last_error = msg;
@@ -55,5 +58,5 @@ extern "C" unsigned cflk_device_status(void) {
     return cflk::read_and_clear_status_fwd() | cflk::read_and_clear_status_bwd() |
            cflk::read_and_clear_status_fused() | cflk::read_and_clear_status_gemm() |
            cflk::read_and_clear_status_opm() | cflk::read_and_clear_status_xent() |
-           cflk::read_and_clear_status_head();
+           cflk::read_and_clear_status_head() | cflk::read_and_clear_status_few();
 }

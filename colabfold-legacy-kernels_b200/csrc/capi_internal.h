@@ -27,6 +27,7 @@ unsigned read_and_clear_status_gemm();
 unsigned read_and_clear_status_opm();
 unsigned read_and_clear_status_xent();
 unsigned read_and_clear_status_head();
+unsigned read_and_clear_status_few();
 
 // VoltaOpmOuter fused at C = E = 32 (the caller has validated the sizes); the workspace holds
 // wT laid out chunk by chunk (F * 2 KB)
@@ -49,6 +50,10 @@ struct HeadCall {
 bool xent_head_fits(int64_t V, int64_t C, bool bwd);
 size_t xent_head_workspace(int64_t T, int64_t V, int64_t C, bool bwd);
 cudaError_t xent_head(const HeadCall& c, bool bwd, bool& map_ok);
+// the forward of a few tokens
+bool xent_few_fits(int64_t T);
+size_t xent_few_workspace();
+cudaError_t xent_few(const HeadCall& c, bool& map_ok);
 
 // VoltaGdp through the tile GEMM (widths the resident-weight row-tile kernel does not take)
 int gdp_general(void* stream, int dtype, const void* x, const void* wp, const void* bp,

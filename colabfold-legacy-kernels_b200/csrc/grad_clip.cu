@@ -31,6 +31,7 @@ constexpr int kChunk = 16384;        // elements
 constexpr int kTable = 900;          // 32 KB of kernel parameters at most
 constexpr float kInfF = __builtin_huge_valf();
 constexpr int kUnroll = 4;           // 16-byte loads a thread keeps in flight
+constexpr int kSumUnroll = 8;
 
 struct Table {
     int n;
@@ -132,15 +133,15 @@ __device__ __forceinline__ double chunk_sumsq(const T* p, long long numel, int a
     const T* q = p + head;
     const long long b = (long long)at_chunk * kChunk;
     const long long e = b + kChunk < body ? b + kChunk : body;
-    for (long long i = b + threadIdx.x * V; i < e; i += (long long)kThreads * V * kUnroll) {
-        Raw<T, V> v[kUnroll];
+    for (long long i = b + threadIdx.x * V; i < e; i += (long long)kThreads * V * kSumUnroll) {
+        Raw<T, V> v[kSumUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < kSumUnroll; ++u) {
             const long long j = i + (long long)u * kThreads * V;
             v[u] = load_raw<T, V>(q + (j < e ? j : i));
         }
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < kSumUnroll; ++u) {
             if (i + (long long)u * kThreads * V < e) {
                 acc += vector_sumsq<T>(v[u]);
             }

@@ -861,7 +861,9 @@ constexpr size_t kPieceBytes = size_t(512) << 20;  // g of one piece of the clas
 constexpr int kPairs = 74;
 
 struct Plan {
-    bool head;         // few classes: xent_head.cu, whose workspace is all it needs
+    // few classes, or (forward) few tokens: xent_head.cu and xent_few.cu, whose workspace is all
+    // they need
+    bool head, few;
     int64_t tp;        // rows of the gathered tokens, whole tiles
     int64_t row_step;  // forward: rows a launch
     int64_t vp;        // classes a piece (backward), whole tiles
@@ -884,6 +886,11 @@ bool make_plan(int64_t T, int64_t V, int64_t C, bool bwd, Plan& p) {
     p.head = xent_head_fits(V, C, bwd);
     if (p.head) {
         p.bytes = xent_head_workspace(T, V, C, bwd);
+        return true;
+    }
+    p.few = !bwd && xent_few_fits(T);
+    if (p.few) {
+        p.bytes = xent_few_workspace();
         return true;
     }
     p.tp = (T + PM - 1) / PM * PM;
@@ -1254,6 +1261,7 @@ extern "C" int cflk_linear_xent(void* stream, int dtype, int labels_64, const vo
     c.workspace = workspace;
     bool map_ok = true;
     const cudaError_t e = p.head           ? xent_head(c, false, map_ok)
+                          : p.few          ? xent_few(c, map_ok)
                           : dtype == kBF16 ? forward<__nv_bfloat16>(c, p, map_ok)
                                            : forward<__half>(c, p, map_ok);
     return finish(who, map_ok, e);
