@@ -28,24 +28,27 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kBlocksPerSm = 4;    // at most 64 registers a thread: all resident at once
 constexpr int kBlocks = 148 * kBlocksPerSm;
 constexpr int kChunk = 16384;        // elements
-constexpr int kTable = 900;          // 32 KB of kernel parameters at most
+constexpr int kTable = 900;          // tensors a launch: 32 KB of kernel parameters at most
+constexpr int kSmallTable = 64;      // and of a call of few, whose parameters cost less to pass
 constexpr float kInfF = __builtin_huge_valf();
 constexpr int kUnroll = 4;           // 16-byte loads a thread keeps in flight
 constexpr int kSumUnroll = 8;
 
+template <int N>
 struct Table {
     int n;
     int chunks;
-    const void* src[kTable];
-    void* dst[kTable];
-    long long numel[kTable];
-    int first[kTable];              // the tensor's first chunk
-    uint8_t type[kTable];           // source type, destination type << 4
+    const void* src[N];
+    void* dst[N];
+    long long numel[N];
+    int first[N];              // the tensor's first chunk
+    uint8_t type[N];           // source type, destination type << 4
 };
-static_assert(sizeof(Table) <= 32000, "kernel parameters");
+static_assert(sizeof(Table<kTable>) <= 32000, "kernel parameters");
 
 // the tensor that holds chunk c: the last with first <= c (tensors without elements have none)
-__device__ __forceinline__ int find_tensor(const Table& t, int c) {
+template <int N>
+__device__ __forceinline__ int find_tensor(const Table<N>& t, int c) {
     int lo = 0, hi = t.n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -151,13 +154,15 @@ __device__ __forceinline__ double chunk_sumsq(const T* p, long long numel, int a
 }
 
 // The chunks of block `b`: a contiguous range, so that a block looks its first tensor up once.
-__device__ __forceinline__ void block_range(const Table& t, int& c0, int& c1) {
+template <int N>
+__device__ __forceinline__ void block_range(const Table<N>& t, int& c0, int& c1) {
     c0 = (int)((long long)t.chunks * blockIdx.x / gridDim.x);
     c1 = (int)((long long)t.chunks * (blockIdx.x + 1) / gridDim.x);
 }
 
+template <int N>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
-    sumsq_kernel(const __grid_constant__ Table t, double* __restrict__ partial) {
+    sumsq_kernel(const __grid_constant__ Table<N> t, double* __restrict__ partial) {
     double acc = 0.0;
     int c0, c1;
     block_range(t, c0, c1);
@@ -252,8 +257,9 @@ __device__ __forceinline__ void chunk_scale(const TI* p, TO* o, long long numel,
 }
 
 // `partial`: the sums of cflk_grad_clip's first launch, or one sumsq (n 1).
+template <int N>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
-    clip_kernel(const __grid_constant__ Table t, const double* __restrict__ partial, int n,
+    clip_kernel(const __grid_constant__ Table<N> t, const double* __restrict__ partial, int n,
                 float max_norm, float eps, float scale, float* __restrict__ norm_out) {
     const double sumsq = sum_partials(partial, n);
     const float norm = (float)(sqrt(sumsq) * fabs((double)scale));
@@ -299,11 +305,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 }
 
 // the tensors from `at` on that one launch takes; the index after them
-int64_t fill_table(Table& t, int64_t at, int64_t n, const void* const* src, void* const* dst,
+template <int N>
+int64_t fill_table(Table<N>& t, int64_t at, int64_t n, const void* const* src, void* const* dst,
                    const int64_t* numel, const int* src_dtype, const int* dst_dtype) {
     t.n = 0;
     t.chunks = 0;
-    for (; at < n && t.n < kTable; ++at) {
+    for (; at < n && t.n < N; ++at) {
         if (numel[at] == 0) {
             continue;
         }
@@ -362,10 +369,11 @@ int check_tensors(const char* who, int64_t n, const void* const* src, void* cons
 }
 
 // The launches of the sum; their number of partials in `parts`.
+template <int N>
 cudaError_t launch_sumsq(cudaStream_t s, int64_t n, const void* const* grads,
                          const int64_t* numel, const int* dtypes, double* partial, int& parts) {
     parts = 0;
-    Table t;
+    Table<N> t;
     for (int64_t at = 0; at < n;) {
         at = fill_table(t, at, n, grads, nullptr, numel, dtypes, nullptr);
         if (t.n == 0) {
@@ -378,11 +386,12 @@ cudaError_t launch_sumsq(cudaStream_t s, int64_t n, const void* const* grads,
     return cudaGetLastError();
 }
 
+template <int N>
 cudaError_t launch_clip(cudaStream_t s, int64_t n, const void* const* grads, void* const* outs,
                         const int64_t* numel, const int* dtypes, const int* out_dtypes,
                         const double* partial, int parts, float max_norm, float eps, float scale,
                         float* norm) {
-    Table t;
+    Table<N> t;
     int64_t at = 0;
     do {
         at = fill_table(t, at, n, grads, outs, numel, dtypes, out_dtypes);
@@ -446,7 +455,8 @@ extern "C" int cflk_grad_sumsq(void* stream, int64_t n, const void* const* grads
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     double* partial = static_cast<double*>(workspace);
     int parts = 0;
-    cudaError_t e = launch_sumsq(s, n, grads, numel, dtypes, partial, parts);
+    cudaError_t e = (n <= kSmallTable ? launch_sumsq<kSmallTable> : launch_sumsq<kTable>)(
+        s, n, grads, numel, dtypes, partial, parts);
     if (e == cudaSuccess) {
         sumsq_final_kernel<<<1, kThreads, 0, s>>>(partial, parts, sumsq);
         e = cudaGetLastError();
@@ -480,11 +490,13 @@ extern "C" int cflk_grad_clip(void* stream, int64_t n, const void* const* grads,
         if (rc != kOk) {
             return rc;
         }
-        e = launch_sumsq(s, n, grads, numel, dtypes, static_cast<double*>(workspace), parts);
+        e = (n <= kSmallTable ? launch_sumsq<kSmallTable> : launch_sumsq<kTable>)(
+            s, n, grads, numel, dtypes, static_cast<double*>(workspace), parts);
         partial = static_cast<const double*>(workspace);
     }
     if (e == cudaSuccess) {
-        e = launch_clip(s, n, grads, outs, numel, dtypes, out_dtypes, partial, parts, max_norm, eps,
+        e = (n <= kSmallTable ? launch_clip<kSmallTable> : launch_clip<kTable>)(
+            s, n, grads, outs, numel, dtypes, out_dtypes, partial, parts, max_norm, eps,
                         scale, norm);
     }
     if (e != cudaSuccess) {

@@ -10,6 +10,9 @@ error RuntimeError. 16-bit tensors may be float16 (the reference's type) or bflo
 There is no fallback: if libcflk_sm100.so is missing or cannot be loaded, every call raises.
 """
 import ctypes
+import functools
+import operator
+from array import array
 
 import torch
 
@@ -118,11 +121,12 @@ def _ptr(t):
         raise ValueError('tensors must be on a CUDA device')
     if not t.is_contiguous():
         raise ValueError('tensors must be contiguous')
-    return _C.c_void_p(t.data_ptr())
+    return t.data_ptr()
 
 
 def _stream():
-    return _C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the current stream's handle, without an object for it
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _f32_ptr(t, name, who):
@@ -568,10 +572,16 @@ def _code(t, name, who):
     return _CODES[t.dtype]
 
 
-def _workspace(size_fn, args, like, who):
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(size_fn, args, who):
     n = _C.c_size_t(0)
     _check(getattr(lib(), size_fn)(*args, _C.byref(n)), who)
-    return torch.empty(max(n.value, 1), dtype=torch.uint8, device=like.device), n.value
+    return n.value
+
+
+def _workspace(size_fn, args, like, who):
+    n = _workspace_bytes(size_fn, args, who)
+    return torch.empty(max(n, 1), dtype=torch.uint8, device=like.device), n
 
 
 def embed(ids, table, *, scale=1.0, out_dtype=None, out=None):
@@ -651,35 +661,41 @@ def linear_xent_bwd(x, w, labels, lse, dloss, bias=None):
     return dx, dw, dbias
 
 
+_dtype_of = operator.attrgetter('dtype')
+
+
 def _tensor_table(tensors, who):
-    """(pointers, element counts, type codes) of contiguous CUDA tensors as C arrays."""
-    n = len(tensors)
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
+    """Addresses, element counts and type codes of contiguous CUDA tensors, as arrays that C reads
+    in place, and their device's index. A call may hold hundreds of tensors: every step is one pass
+    of a built-in over the list."""
+    T = torch.Tensor
+    if not all(map(T.is_contiguous, tensors)):
         raise ValueError('%s: tensors must be contiguous' % who)
     try:
-        codes = [_CODES[t.dtype] for t in tensors]
+        codes = array('i', map(_CODES.__getitem__, map(_dtype_of, tensors)))
     except KeyError as e:
         raise ValueError('%s: gradients must be float16, bfloat16 or float32, got %s' %
                          (who, e)) from None
-    if len({t.device for t in tensors}) > 1 or (n and not tensors[0].is_cuda):
+    devices = set(map(T.get_device, tensors))
+    if len(devices) > 1 or (devices and min(devices) < 0):
         raise ValueError('%s: tensors must be on one CUDA device' % who)
-    return ((_p * n)(*map(torch.Tensor.data_ptr, tensors)),
-            (_i64 * n)(*map(torch.Tensor.numel, tensors)), (_int * n)(*codes))
+    return (array('q', map(T.data_ptr, tensors)), array('q', map(T.numel, tensors)), codes,
+            devices.pop() if devices else torch.cuda.current_device())
 
 
-def _grad_device(grads):
-    return grads[0].device if grads else torch.device('cuda', torch.cuda.current_device())
+def _at(a):
+    return a.buffer_info()[0]
 
 
 def grad_sumsq(grads):
     """The sum of the squares of all elements of the tensors: float64 [1] on their device."""
     who = 'grad_norm'
     grads = list(grads)
-    ptrs, numel, codes = _tensor_table(grads, who)
-    out = torch.empty(1, dtype=torch.float64, device=_grad_device(grads))
+    ptrs, numel, codes, device = _tensor_table(grads, who)
+    out = torch.empty(1, dtype=torch.float64, device=device)
     ws, nb = _workspace('cflk_grad_workspace_size', (len(grads),), out, who)
-    _check(lib().cflk_grad_sumsq(_stream(), len(grads), ptrs, numel, codes, _ptr(out), _ptr(ws),
-                                 nb), who)
+    _check(lib().cflk_grad_sumsq(_stream(), len(grads), _at(ptrs), _at(numel), _at(codes),
+                                 _ptr(out), _ptr(ws), nb), who)
     return out
 
 
@@ -690,16 +706,18 @@ def clip_grad_norm(grads, max_norm, *, scale=1.0, eps=1e-6, out=None, sumsq=None
     of squares to use instead of these tensors' own, as the ranks of a sharded model add it up."""
     who = 'grad_clip'
     grads = list(grads)
-    outs = grads if out is None else list(out)
-    if len(outs) != len(grads) or any(o.numel() != g.numel() for o, g in zip(outs, grads)):
-        raise ValueError('grad_clip: out must hold a tensor of the same size for each gradient')
-    ptrs, numel, codes = _tensor_table(grads, who)
-    optrs, _, ocodes = (ptrs, numel, codes) if out is None else _tensor_table(outs, who)
-    norm = torch.empty((), dtype=torch.float32, device=_grad_device(grads))
+    ptrs, numel, codes, device = _tensor_table(grads, who)
+    optrs, onumel, ocodes = ptrs, numel, codes
+    if out is not None:
+        optrs, onumel, ocodes, odevice = _tensor_table(list(out), who)
+        if onumel != numel or odevice != device:
+            raise ValueError(
+                'grad_clip: out must hold a tensor of the same size and device for each gradient')
+    norm = torch.empty((), dtype=torch.float32, device=device)
     if sumsq is not None and (sumsq.dtype != torch.float64 or sumsq.numel() != 1):
         raise ValueError('grad_clip: sumsq must be one float64')
     ws, nb = _workspace('cflk_grad_workspace_size', (len(grads),), norm, who)
-    _check(lib().cflk_grad_clip(_stream(), len(grads), ptrs, optrs, numel, codes, ocodes,
-                                _ptr(sumsq), float(max_norm), float(eps), float(scale),
+    _check(lib().cflk_grad_clip(_stream(), len(grads), _at(ptrs), _at(optrs), _at(numel),
+                                _at(codes), _at(ocodes), _ptr(sumsq), float(max_norm), float(eps), float(scale),
                                 _ptr(norm), _ptr(ws), nb), who)
     return norm
