@@ -118,11 +118,50 @@ __device__ __forceinline__ unsigned sort_key(const Id* ids, long long t, unsigne
     return id >= 0 && id < (long long)V ? (unsigned)id : V;
 }
 
+// Rows without a token get zeros. The first kernel of the sort marks the rows that have one in a
+// bitmap; the kernels after it, whose own blocks leave most SMs idle, each carry blocks that write
+// a share of the others.
+struct ZeroShare {
+    const unsigned* present;  // a bit a row
+    float* dtable;
+    int row0, row1;           // rows of this launch, multiples of 32 (or V)
+    int C, blocks;            // channels; blocks at the end of the grid
+    int vec;
+};
+
+// `block` of s.blocks, `warps` warps a block: 32 rows a block a step, its warps in turn
+__device__ __forceinline__ void zero_rows(const ZeroShare& s, int block, int warps) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int r0 = s.row0 + block * 32; r0 < s.row1; r0 += s.blocks * 32) {
+        const unsigned present = s.present[r0 >> 5];
+        for (int r = warp; r < min(32, s.row1 - r0); r += warps) {
+            if ((present >> r) & 1) {
+                continue;
+            }
+            float* dst = s.dtable + (long long)(r0 + r) * s.C;
+            if (s.vec) {
+                for (int c = lane * 4; c < s.C; c += 128) {
+                    *reinterpret_cast<float4*>(dst + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            } else {
+                for (int c = lane; c < s.C; c += 32) {
+                    dst[c] = 0.f;
+                }
+            }
+        }
+    }
+}
+
 // counts[digit][block]
 template <typename Key>
 __global__ void __launch_bounds__(kSortThreads)
     sort_count_kernel(const Key* __restrict__ keys, int T, unsigned V, int shift, int bits,
-                      int* __restrict__ counts, int nblocks) {
+                      int* __restrict__ counts, int nblocks, unsigned* __restrict__ mark,
+                      const ZeroShare zero) {
+    if ((int)blockIdx.x >= nblocks) {
+        zero_rows(zero, blockIdx.x - nblocks, kSortWarps);
+        return;
+    }
     __shared__ int hist[1 << kMaxDigit];
     const int bins = 1 << bits;
     for (int i = threadIdx.x; i < bins; i += kSortThreads) {
@@ -133,7 +172,11 @@ __global__ void __launch_bounds__(kSortThreads)
     for (int j = 0; j < kSortRounds; ++j) {
         const long long t = (long long)blockIdx.x * kSortItems + j * kSortThreads + threadIdx.x;
         if (t < T) {
-            atomicAdd(&hist[(sort_key(keys, t, V) >> shift) & (bins - 1)], 1);
+            const unsigned key = sort_key(keys, t, V);
+            atomicAdd(&hist[(key >> shift) & (bins - 1)], 1);
+            if (mark != nullptr && key < V) {
+                atomicOr(&mark[key >> 5], 1u << (key & 31));
+            }
         }
     }
     __syncthreads();
@@ -181,8 +224,12 @@ __global__ void __launch_bounds__(kSortThreads)
     sort_scatter_kernel(const Key* __restrict__ keys, const int* __restrict__ toks, int T,
                         unsigned V, int shift, int bits, const int* __restrict__ counts,
                         const int* __restrict__ totals, int nblocks, int scanned,
-                        unsigned* __restrict__ okeys,
-                        int* __restrict__ otoks) {
+                        unsigned* __restrict__ okeys, int* __restrict__ otoks,
+                        const ZeroShare zero) {
+    if ((int)blockIdx.x >= nblocks) {
+        zero_rows(zero, blockIdx.x - nblocks, kSortWarps);
+        return;
+    }
     __shared__ int run[kSortWarps][1 << kMaxDigit];
     __shared__ int base[1 << kMaxDigit];
     __shared__ int warp_sum[kSortWarps];
@@ -292,60 +339,21 @@ __global__ void __launch_bounds__(kSortThreads)
 // ------------------------------------------------------------------------------------------
 constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
 
-// Rows without a token get zeros: 32 rows a warp a step, each lane looks its row up in the sorted
-// keys.
-template <int VEC>
-__device__ __forceinline__ void zero_rows(const unsigned* keys, float* dtable, int n, unsigned V,
-                                          int C, long long warp, long long warps) {
-    const int lane = threadIdx.x & 31;
-    for (long long r0 = warp * 32; r0 < (long long)V; r0 += warps * 32) {
-        const long long row = r0 + lane;
-        bool empty = row < (long long)V;
-        if (empty) {
-            int lo = 0, hi = n;  // first place with keys >= row
-            while (lo < hi) {
-                const int mid = (int)(((long long)lo + hi) >> 1);
-                if (keys[mid] < (unsigned)row) {
-                    lo = mid + 1;
-                } else {
-                    hi = mid;
-                }
-            }
-            empty = lo >= n || keys[lo] != (unsigned)row;
-        }
-        unsigned todo = __ballot_sync(0xffffffffu, empty);
-        float zero[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            zero[i] = 0.f;
-        }
-        while (todo != 0) {
-            const int r = __ffs(todo) - 1;
-            todo &= todo - 1;
-            float* dst = dtable + (r0 + r) * C;
-            for (int col = lane * VEC; col < C; col += 32 * VEC) {
-                store_vec<float, VEC>(dst + col, zero);
-            }
-        }
-    }
-}
-
 // A warp sums chunk `c` of the sorted list (len pairs) over one slab of 32 VEC channels. Rows
 // whose pairs all lie in the chunk are written; the sum of a row that began before the chunk goes
 // to partial[c][0], that of a row that began in it and goes on after it to partial[c][1]. The
-// blocks past the first sum_blocks write the rows without a token meanwhile.
+// blocks past the first sum_blocks write their share of the rows without a token.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSumThreads)
     embed_sum_kernel(const unsigned* __restrict__ keys, const int* __restrict__ toks,
                      const T* __restrict__ dout, float* __restrict__ dtable,
                      float* __restrict__ partial, int n, unsigned V, int C, int slabs, int chunks,
-                     int len, int sum_blocks, float scale) {
+                     int len, int sum_blocks, float scale, const ZeroShare zero) {
     constexpr int kUnroll = 8;
     const int lane = threadIdx.x & 31;
     const long long item = (long long)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
     if ((int)blockIdx.x >= sum_blocks) {
-        zero_rows<VEC == 1 ? 1 : 4>(keys, dtable, n, V, C, item - (long long)sum_blocks * kSumWarps,
-                       (long long)(gridDim.x - sum_blocks) * kSumWarps);
+        zero_rows(zero, blockIdx.x - sum_blocks, kSumWarps);
         return;
     }
     if (item >= (long long)chunks * slabs) {
@@ -418,46 +426,23 @@ __global__ void __launch_bounds__(kSumThreads)
     flush(true);
 }
 
-// Rows that cross a chunk's end, by the warp of the chunk they begin in: its part and the
-// following chunks' in order.
+// Rows that cross a chunk's end, by the chunk they begin in: its part and the following chunks' in
+// order. A warp an item (chunk, slab); rows of more than kLong parts by the block's warps together, each
+// a contiguous share of the parts.
+constexpr int kLong = 9;
+
 template <int VEC>
-__device__ __forceinline__ void join_row(const unsigned* keys, float* dtable,
-                                         const float* partial, int n, unsigned V, int C, int c,
-                                         int slab, int len, float scale) {
-    const int lane = threadIdx.x & 31, col = (slab * 32 + lane) * VEC;
-    const long long end = (long long)(c + 1) * len;
-    if (end >= n) {
-        return;
-    }
-    const unsigned row = keys[end - 1];
-    const bool began_here = c == 0 || keys[(long long)c * len - 1] != row;
-    if (row >= V || keys[end] != row || !began_here || col >= C) {
-        return;
-    }
-    // the row's last chunk: the one that holds the last pair with its key
-    long long lo = end, hi = n;  // keys[lo] == row, keys[hi] != row (or past the end)
-    while (hi - lo > 1) {
-        const long long mid = (lo + hi) >> 1;
-        if (keys[mid] == row) {
-            lo = mid;
-        } else {
-            hi = mid;
-        }
-    }
-    const int last = (int)(lo / len);
-    float acc[VEC];
-    load_vec<float, VEC>(partial + ((long long)c * 2 + 1) * C + col, acc);
-    for (int q = c + 1; q <= last; q += 8) {
+__device__ __forceinline__ void add_parts(const float* partial, int q0, int q1, int C, int col,
+                                          float (&acc)[VEC]) {
+    for (int q = q0; q < q1; q += 8) {
         float v[8][VEC];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            if (q + u <= last) {
-                load_vec<float, VEC>(partial + (long long)(q + u) * 2 * C + col, v[u]);
-            }
+            load_vec<float, VEC>(partial + (long long)min(q + u, q1 - 1) * 2 * C + col, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            if (q + u <= last) {
+            if (q + u < q1) {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     acc[i] += v[u][i];
@@ -465,11 +450,6 @@ __device__ __forceinline__ void join_row(const unsigned* keys, float* dtable,
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        acc[i] *= scale;
-    }
-    store_vec<float, VEC>(dtable + (long long)row * C + col, acc);
 }
 
 template <int VEC>
@@ -477,11 +457,91 @@ __global__ void __launch_bounds__(kSumThreads)
     embed_join_kernel(const unsigned* __restrict__ keys, float* __restrict__ dtable,
                       const float* __restrict__ partial, int n, unsigned V, int C, int slabs,
                       int chunks, int len, float scale) {
-    const long long item = (long long)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
+    __shared__ int long_last[kSumWarps];  // the last chunk of a warp's long row, or -1
+    __shared__ __align__(32) float part_sum[kSumWarps][32 * VEC];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long item0 = (long long)blockIdx.x * kSumWarps;
+    // (chunks fastest: the slabs of a long row fall to different blocks)
+    const auto column = [&](long long item) {
+        return ((int)(item / chunks) * 32 + lane) * VEC;
+    };
+    const long long item = item0 + warp;
+    int last = -1;
     if (item < (long long)chunks * slabs) {
-        const int c = (int)(item / slabs);
-        join_row<VEC>(keys, dtable, partial, n, V, C, c, (int)(item - (long long)c * slabs), len,
-                      scale);
+        const int c = (int)(item % chunks);
+        const long long end = (long long)(c + 1) * len;
+        // a row that begins in chunk c and goes on: its following chunks, 32 looks at a time
+        if (end < n) {
+            const unsigned row = keys[end - 1];
+            const unsigned before = c > 0 ? keys[(long long)c * len - 1] : 0xffffffffu;
+            if (row < V && before != row && keys[end] == row) {
+                last = c;
+                for (int q = c + 1; q < chunks; q += 32) {
+                    const long long at = (long long)(q + lane) * len;
+                    const unsigned same =
+                        __ballot_sync(0xffffffffu, q + lane < chunks && keys[min(at, n - 1ll)] == row);
+                    const int run = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+                    last += run;
+                    if (run < 32) {
+                        break;
+                    }
+                }
+                const int col = column(item);
+                if (last - c < kLong && col < C) {
+                    float acc[VEC];
+                    load_vec<float, VEC>(partial + ((long long)c * 2 + 1) * C + col, acc);
+                    add_parts<VEC>(partial, c + 1, last + 1, C, col, acc);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        acc[i] *= scale;
+                    }
+                    store_vec<float, VEC>(dtable + (long long)row * C + col, acc);
+                }
+                last = last - c < kLong ? -1 : last;
+            }
+        }
+    }
+    if (lane == 0) {
+        long_last[warp] = last;
+    }
+    __syncthreads();
+    for (int w = 0; w < kSumWarps; ++w) {
+        if (long_last[w] < 0) {
+            continue;
+        }
+        const int c = (int)((item0 + w) % chunks), col = column(item0 + w), parts = long_last[w] - c;
+        const bool on = col < C;
+        float acc[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            acc[i] = 0.f;
+        }
+        if (on) {
+            if (warp == 0) {
+                load_vec<float, VEC>(partial + ((long long)c * 2 + 1) * C + col, acc);
+            }
+            add_parts<VEC>(partial, c + 1 + parts * warp / kSumWarps,
+                           c + 1 + parts * (warp + 1) / kSumWarps, C, col, acc);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            part_sum[warp][lane * VEC + i] = acc[i];
+        }
+        __syncthreads();
+        if (warp == 0 && on) {
+            for (int k = 1; k < kSumWarps; ++k) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    acc[i] += part_sum[k][lane * VEC + i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                acc[i] *= scale;
+            }
+            store_vec<float, VEC>(dtable + (long long)keys[(long long)(c + 1) * len] * C + col, acc);
+        }
+        __syncthreads();
     }
 }
 
@@ -736,7 +796,7 @@ struct BwdPlan {
     long long per;     // tokens a CTA
     int passes, bits, nblocks;
     int slabs, chunks, len, vec;
-    size_t off_counts, off_totals, off_keys[2], off_toks[2], off_partial, bytes;
+    size_t off_present, off_counts, off_totals, off_keys[2], off_toks[2], off_partial, bytes;
 };
 
 size_t round256(size_t n) {
@@ -780,6 +840,7 @@ bool plan_bwd(int64_t T, int64_t V, int64_t C, int vec, BwdPlan& p) {
         at += round256(n);
         return o;
     };
+    p.off_present = take((size_t)(V + 31) / 32 * 4);
     p.off_counts = take((size_t)p.nblocks * (size_t(1) << p.bits) * 4);
     p.off_totals = take((size_t(1) << p.bits) * 4);
     for (int i = 0; i < 2; ++i) {
@@ -840,6 +901,26 @@ cudaError_t launch_embed_bwd(cudaStream_t s, const void* ids, const void* dout, 
         toks[i] = reinterpret_cast<int*>(ws + p.off_toks[i]);
     }
     float* partial = reinterpret_cast<float*>(ws + p.off_partial);
+    unsigned* present = reinterpret_cast<unsigned*>(ws + p.off_present);
+    cudaError_t e = cudaMemsetAsync(present, 0, (size_t)(V + 31) / 32 * 4, s);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    // the rows without a token in equal shares, one for every kernel after the first but the scans
+    const int shares = 2 * p.passes;
+    int share = 0;
+    const auto next_share = [&] {
+        ZeroShare z{};
+        z.present = present;
+        z.dtable = dtable;
+        z.row0 = (int)(V * share / shares / 32 * 32);
+        ++share;
+        z.row1 = share == shares ? (int)V : (int)(V * share / shares / 32 * 32);
+        z.C = (int)C;
+        z.vec = p.vec > 1;
+        z.blocks = std::min(8 * kSms, (z.row1 - z.row0 + 31) / 32);
+        return z;
+    };
     const int bins = 1 << p.bits;
     int cur = 0;
     for (int pass = 0; pass < p.passes; ++pass) {
@@ -847,41 +928,45 @@ cudaError_t launch_embed_bwd(cudaStream_t s, const void* ids, const void* dout, 
         if (pass == 0) {
             sort_count_kernel<Id><<<p.nblocks, kSortThreads, 0, s>>>(
                 static_cast<const Id*>(ids), (int)n, (unsigned)V, shift, p.bits, counts,
-                p.nblocks);
+                p.nblocks, present, ZeroShare{});
         } else {
-            sort_count_kernel<unsigned><<<p.nblocks, kSortThreads, 0, s>>>(
-                keys[cur], (int)n, (unsigned)V, shift, p.bits, counts, p.nblocks);
+            const ZeroShare z = next_share();
+            sort_count_kernel<unsigned><<<p.nblocks + z.blocks, kSortThreads, 0, s>>>(
+                keys[cur], (int)n, (unsigned)V, shift, p.bits, counts, p.nblocks, nullptr, z);
         }
         const int scanned = p.nblocks > kFewBlocks;
         if (scanned) {
             sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(
                 counts, totals, bins, p.nblocks);
         }
+        const ZeroShare z = next_share();
         if (pass == 0) {
-            sort_scatter_kernel<Id, true><<<p.nblocks, kSortThreads, 0, s>>>(
+            sort_scatter_kernel<Id, true><<<p.nblocks + z.blocks, kSortThreads, 0, s>>>(
                 static_cast<const Id*>(ids), nullptr, (int)n, (unsigned)V, shift, p.bits, counts,
-                totals, p.nblocks, scanned, keys[cur], toks[cur]);
+                totals, p.nblocks, scanned, keys[cur], toks[cur], z);
         } else {
-            sort_scatter_kernel<unsigned, false><<<p.nblocks, kSortThreads, 0, s>>>(
+            sort_scatter_kernel<unsigned, false><<<p.nblocks + z.blocks, kSortThreads, 0, s>>>(
                 keys[cur], toks[cur], (int)n, (unsigned)V, shift, p.bits, counts, totals,
-                p.nblocks, scanned, keys[cur ^ 1], toks[cur ^ 1]);
+                p.nblocks, scanned, keys[cur ^ 1], toks[cur ^ 1], z);
             cur ^= 1;
         }
     }
     const int64_t items = (int64_t)p.chunks * p.slabs;
     const unsigned sum_grid = (unsigned)((items + kSumWarps - 1) / kSumWarps);
-    // blocks for the rows without a token
-    const unsigned zero_grid = (unsigned)std::min<int64_t>(
-        4 * kSms, (V + 32 * kSumWarps - 1) / (32 * kSumWarps));
+    const ZeroShare z = next_share();
     const auto sum = [&](auto tag) {
         constexpr int VEC = decltype(tag)::value;
-        embed_sum_kernel<T, VEC><<<sum_grid + zero_grid, kSumThreads, 0, s>>>(
+        embed_sum_kernel<T, VEC><<<sum_grid + z.blocks, kSumThreads, 0, s>>>(
             keys[cur], toks[cur], static_cast<const T*>(dout), dtable, partial, (int)n,
-            (unsigned)V, (int)C, p.slabs, p.chunks, p.len, (int)sum_grid, scale);
+            (unsigned)V, (int)C, p.slabs, p.chunks, p.len, (int)sum_grid, scale, z);
         if (p.chunks > 1) {
-            embed_join_kernel<VEC><<<sum_grid, kSumThreads, 0, s>>>(
-                keys[cur], dtable, partial, (int)n, (unsigned)V, (int)C, p.slabs, p.chunks, p.len,
-                scale);
+            constexpr int JVEC = VEC == 1 ? 1 : 4;  // narrower slabs: more blocks for a long row
+            const int slabs = (int)((C + 32 * JVEC - 1) / (32 * JVEC));
+            const int64_t joins = (int64_t)p.chunks * slabs;
+            embed_join_kernel<JVEC>
+                <<<(unsigned)((joins + kSumWarps - 1) / kSumWarps), kSumThreads, 0, s>>>(
+                    keys[cur], dtable, partial, (int)n, (unsigned)V, (int)C, slabs, p.chunks,
+                    p.len, scale);
         }
     };
     if (p.vec == 8) {
