@@ -405,13 +405,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         }
     } else if (warp == 1 && lane == 0 && rank == 0) {
         const uint32_t idesc = idesc_f16(E::kBf16, PM, PN, A_MN, B_MN);
-        // K-major: rows of 128 bytes (8-row groups 1 KB apart), a K step of 16 is 32 bytes along
-        // the row; MN-major: 64-wide atoms 8 KB apart, a K step is 16 rows of 128 bytes
-        const auto desc = [](uint32_t base, int ks, bool mn) -> uint64_t {
-            return mn ? smem_desc(base + ks * 16 * 128, 64 * 128, 1024, kSwizzle128B)
-                      : smem_desc(base + 32 * ks, 16, 1024, kSwizzle128B);
-        };
-        int g = 0, lt = 0;
+        // Descriptors of 128-byte-swizzled operands, 8-row groups 1 KB apart. K-major: a K step of 16
+        // is 32 bytes along the row; MN-major: 64-wide atoms 8 KB apart, a K step is 16 rows of
+        // 128 bytes. The low word holds the address and the atoms' distance in 16-byte units.
+        constexpr uint32_t kHi = (1024 >> 4) | 1u << 14 | (uint32_t)kSwizzle128B << 29;
+        constexpr uint32_t kAStep = A_MN ? 128 : 2, kBStep = B_MN ? 128 : 2;
+        const uint32_t lo0 = smem_u32(smem) >> 4;
+        const uint32_t a0 = lo0 | (uint32_t)(A_MN ? 8192 >> 4 : 1) << 16;
+        const uint32_t b0 = (lo0 + (kHalfBytes >> 4)) | (uint32_t)(B_MN ? 8192 >> 4 : 1) << 16;
+        int s = 0, lt = 0;
+        uint32_t phase = 0;
         bool ok = true;
         for (long long i = pair0; ok && i < items; i += pairs) {
             const Item it = sched.at(i);
@@ -425,21 +428,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             }
             tc_fence_after();
             const uint32_t acc = tmem + buf * PN;
-            for (int kb = it.kb0; kb < it.kb1; ++kb, ++g) {
-                const int s = g % kStages;
-                if (!mbar_wait(&full[s], (g / kStages) & 1, &g_status, kStatusTmaWait,
-                               &abort_flag)) {
+            for (int kb = it.kb0; kb < it.kb1; ++kb) {
+                if (!mbar_wait(&full[s], phase, &g_status, kStatusTmaWait, &abort_flag)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t sa = smem_u32(smem + s * kStageBytes), sb = sa + kHalfBytes;
-#pragma unroll
-                for (int ks = 0; ks < PK / 16; ++ks) {
-                    mma_ss_pair(acc, desc(sa, ks, A_MN), desc(sb, ks, B_MN), idesc,
-                                kb > it.kb0 || ks > 0 ? 1u : 0u);
-                }
+                const uint32_t at = s * (kStageBytes >> 4);
+                mma_pair_k4<kAStep, kBStep, kHi>(acc, a0 + at, b0 + at, idesc, kb > it.kb0);
                 mma_commit_pair(&empty[s]);
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
             if (ok) {
                 mma_commit_pair(&acc_full[buf]);
@@ -518,18 +519,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     }
                     uint32_t v[32];
                     load(ch, v);
-                    float y[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        y[j] = __uint_as_float(v[j]);
-                    }
-                    if (a.bias != nullptr) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            y[j] += bias_sh[g][32 * ch + j];
-                        }
-                    }
-                    row_stats(y, c0, limit, lab, m, s, at_label);
+                    row_stats<32>(v, c0, limit, lab,
+                                  a.bias != nullptr ? &bias_sh[g][32 * ch] : nullptr, m, s,
+                                  at_label);
                 }
                 if (lab >= col0 && lab < min(col0 + 128, limit)) {
                     a.lab_logit[row + a.row0] = at_label;
@@ -550,7 +542,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                         uint32_t v[32];
                         load(2 * j + h, v);
                         float y[32];
-                        row_grad(v, y, c0, limit, grad,
+                        row_grad<32>(v, y, c0, limit, grad,
                                  a.bias != nullptr ? &bias_sh[g][64 * j + 32 * h] : nullptr);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {

@@ -44,37 +44,56 @@ __device__ __forceinline__ float grad_scale(float m) {
     return exp2f((float)min(14 - e, 126));
 }
 
-// 32 logits of a row, columns c0.. of V, into its log2-domain maximum m and sum s (relative to m);
-// at_label takes the label's logit. Columns past V count as -inf; where nothing is left m stays -inf
-// and s 0.
-__device__ __forceinline__ void row_stats(float (&y)[32], int c0, int V, int label, float& m,
-                                          float& s, float& at_label) {
-    if (c0 + 32 > V) {
+// N accumulators of a row (columns c0.. of V; `bias`, or null, their biases in shared memory, 16-byte
+// aligned) into its log2-domain maximum m and sum s (relative to m); at_label takes the label's
+// logit. Columns past V count as -inf; where nothing is left m stays -inf and s 0.
+template <int N>
+__device__ __forceinline__ void row_stats(const uint32_t (&v)[N], int c0, int V, int label,
+                                          const float* bias, float& m, float& s,
+                                          float& at_label) {
+    float y[N];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+    for (int j = 0; j < N; ++j) {
+        y[j] = __uint_as_float(v[j]);
+    }
+    if (bias != nullptr) {
+#pragma unroll
+        for (int q = 0; q < N / 4; ++q) {
+            const float4 b = reinterpret_cast<const float4*>(bias)[q];
+            y[4 * q] += b.x;
+            y[4 * q + 1] += b.y;
+            y[4 * q + 2] += b.z;
+            y[4 * q + 3] += b.w;
+        }
+    }
+    if (c0 + N > V) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
             y[j] = c0 + j < V ? y[j] : -kInf;
         }
     }
     const int at = label - c0;
-    if (at >= 0 && at < 32) {
+    if (at >= 0 && at < N) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < N; ++j) {
             at_label = j == at ? y[j] : at_label;
         }
     }
     float top = y[0];
 #pragma unroll
-    for (int j = 1; j + 1 < 32; j += 2) {
+    for (int j = 1; j + 1 < N; j += 2) {
         top = max3(top, y[j], y[j + 1]);
     }
-    top = fmaxf(top, y[31]);
+    top = fmaxf(top, y[N - 1]);
     const float m1 = fmaxf(m, top * kLog2e);
     const float ref = m1 == -kInf ? 0.f : m1;
+    const uint64_t log2e = pk2(kLog2e, kLog2e), off = pk2(-ref, -ref);
     float part0 = 0.f, part1 = 0.f;
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-        part0 += ex2(fmaf(y[j], kLog2e, -ref));
-        part1 += ex2(fmaf(y[j + 1], kLog2e, -ref));
+    for (int j = 0; j < N; j += 2) {
+        const float2 e = upk2(fma2(pk2(y[j], y[j + 1]), log2e, off));
+        part0 += ex2(e.x);
+        part1 += ex2(e.y);
     }
     s = s * ex2(m - ref) + (part0 + part1);
     m = m1;
@@ -93,13 +112,14 @@ struct GradRow {
     }
 };
 
-// 32 accumulators of a row, columns c0.. of V, to g; `bias` (or null) is their 32 biases in shared
-// memory. Columns past V give zeros. Pairs of columns share an instruction where they can.
-__device__ __forceinline__ void row_grad(const uint32_t (&v)[32], float (&y)[32], int c0, int V,
+// N accumulators of a row to g, as row_stats takes them. Columns past V give zeros. Pairs of
+// columns share an instruction where they can.
+template <int N>
+__device__ __forceinline__ void row_grad(const uint32_t (&v)[N], float (&y)[N], int c0, int V,
                                          const GradRow& row, const float* bias) {
     const uint64_t log2e = pk2(kLog2e, kLog2e), ref = pk2(-row.lse2, -row.lse2);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
+    for (int q = 0; q < N / 4; ++q) {
         uint64_t l0 = pk2(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]));
         uint64_t l1 = pk2(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3]));
         if (bias != nullptr) {
@@ -114,10 +134,10 @@ __device__ __forceinline__ void row_grad(const uint32_t (&v)[32], float (&y)[32]
         y[4 * q + 3] = ex2(e1.y);
     }
     const int at = row.label - c0;
-    if (at >= 0 && at < 32) {
+    if (at >= 0 && at < N) {
         const unsigned bit = 1u << at;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < N; ++j) {
             if (bit & (1u << j)) {
                 y[j] -= 1.f;
             }
@@ -125,14 +145,14 @@ __device__ __forceinline__ void row_grad(const uint32_t (&v)[32], float (&y)[32]
     }
     const uint64_t dl = pk2(row.dl, row.dl);
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
+    for (int q = 0; q < N / 2; ++q) {
         const float2 g = upk2(mul2(pk2(y[2 * q], y[2 * q + 1]), dl));
         y[2 * q] = g.x;
         y[2 * q + 1] = g.y;
     }
-    if (c0 + 32 > V) {
+    if (c0 + N > V) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < N; ++j) {
             y[j] = c0 + j < V ? y[j] : 0.f;
         }
     }

@@ -14,7 +14,7 @@
 //     N-major B of dx; a tile of x, gathered row by row by four warps' asynchronous copies, is the
 //     K-major A of the logits, then the N-major B of dw; g is the K-major A of dx and the M-major
 //     A of dw;
-//   * two warpgroups take the tiles in turn, each with its own tensor-memory slot, so one's
+//   * four warpgroups work on two tiles (forward: four), each tile with its own tensor-memory slot, so one's
 //     exponentials overlap the other's products and stores; each has a warp that issues its
 //     MMAs, and dw's are issued in the order of the tiles;
 //   * each CTA leaves a float32 dw (and dbias), a second kernel adds them in order: the same bits
@@ -43,10 +43,10 @@ namespace {
 
 __device__ unsigned g_status;
 
-// two warpgroups of workers, then, a warp for each of them, the column sums of g (dbias), the MMAs;
+// four warpgroups of workers; a warp for each tile at work: the column sums of g (dbias), the MMAs;
 // and four loading warps
-constexpr int kThreads = 512;
-constexpr int kSumWarp = 8, kMmaWarp = 10, kLoad0 = 12, kLoaders = 4;
+constexpr int kThreads = 768;
+constexpr int kSumWarp = 16, kMmaWarp = 18, kLoad0 = 20, kLoaders = 4;
 constexpr int kFwdSlots = 4;  // of logits in tensor memory
 constexpr int kRoundBlocks = 32;      // blocks of 128 tokens a CTA lists at a time
 constexpr int kRound = kRoundBlocks * 128;
@@ -171,15 +171,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 4; ++i) {
                 mbar_init(&x_full[i], 32 * kLoaders / l.nx);  // the loading warps' lanes
                 mbar_init(&x_free[i], 1);
-                // a worker warp arrives once
-                mbar_init(&dx_ready[i], 4);
+                // a worker warp arrives once: eight a tile (backward) or four
+                mbar_init(&dx_ready[i], 8);
             }
             for (int i = 0; i < kFwdSlots; ++i) {
                 mbar_init(&l_full[i], 1);
-                mbar_init(&d_free[i], 4);
+                mbar_init(&d_free[i], BWD ? 8 : 4);
             }
             for (int i = 0; i < 2; ++i) {
-                mbar_init(&g_full[i], 4);
+                mbar_init(&g_full[i], 8);
                 mbar_init(&g_free[i], 1);
                 mbar_init(&d_full[i], 1);
                 mbar_init(&dw_done[i], 1);
@@ -581,10 +581,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else if (warp < kSumWarp) {
-            const int h = warp >> 2;                       // warpgroup
+            // forward: a warpgroup a tile; backward: two, half of the columns each
+            const int h = BWD ? (warp >> 2) & 1 : warp >> 2;
+            [[maybe_unused]] const int half = warp >> 3;
             const int r = ((warp & 3) << 5) | lane;        // row of the tile, tensor-memory lane
 #pragma unroll 1
-            for (int c = (base + h) & 1; c < n; c += 2) {
+            for (int c = BWD ? (base + h) & 1 : (h - base) & 3; c < n; c += BWD ? 2 : 4) {
                 const int g = base + c;
                 const int sl = BWD ? h : g % kFwdSlots, turn = BWD ? g >> 1 : g / kFwdSlots;
                 const uint32_t slot = logits_col(sl) + tmem_lane_base(warp);
@@ -613,16 +615,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (!BWD) {
                     float m = -kInf, s = 0.f, at_label = 0.f;
 #pragma unroll 1
-                    for (int c0 = 0; c0 < a.V; c0 += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(slot + c0, v);
+                    for (int c0 = 0; c0 < a.V; c0 += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(slot + c0, v);
                         tmem_wait_ld();
-                        float y[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            y[j] = __uint_as_float(v[j]) + bias_sh[c0 + j];
-                        }
-                        row_stats(y, c0, a.V, lab, m, s, at_label);
+                        row_stats<16>(v, c0, a.V, lab, a.bias != nullptr ? bias_sh + c0 : nullptr,
+                                      m, s, at_label);
                     }
                     tc_fence_before();
                     arrive_warp(&d_free[sl]);
@@ -637,9 +635,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int b = g & nmask;
                     uint8_t* xrow = xs + b * xbytes + r * 128;
 #pragma unroll 1
-                    for (int c0 = 0; c0 < vn; c0 += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(slot + c0, v);
+                    for (int c0 = 16 * half; c0 < vn; c0 += 32) {
+                        uint32_t v[16];
+                        tmem_ld16(slot + c0, v);
                         tmem_wait_ld();
                         if (dense && !live && c0 == 0 && !isfinite(__uint_as_float(v[0]))) {
                             // a row without a label may hold anything, and dw multiplies it by
@@ -651,13 +649,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     make_uint4(0, 0, 0, 0);
                             }
                         }
-                        float y[32];
-                        row_grad(v, y, c0, a.V, grad, a.bias != nullptr ? bias_sh + c0 : nullptr);
+                        float y[16];
+                        row_grad<16>(v, y, c0, a.V, grad,
+                                     a.bias != nullptr ? bias_sh + c0 : nullptr);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
+                        for (int q = 0; q < 2; ++q) {
                             *reinterpret_cast<uint4*>(
                                 grow + (c0 >> 6) * kAtom +
-                                (((((c0 >> 3) & 4) + q) ^ (r & 7)) << 4)) =
+                                (((((c0 >> 3) & 7) + q) ^ (r & 7)) << 4)) =
                                 make_uint4(E::pack(y[8 * q], y[8 * q + 1]),
                                            E::pack(y[8 * q + 2], y[8 * q + 3]),
                                            E::pack(y[8 * q + 4], y[8 * q + 5]),
@@ -683,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                       &abort_flag);
                         }
 #pragma unroll 1
-                        for (int c0 = 0; c0 < end; c0 += 32) {
+                        for (int c0 = 32 * half; c0 < end; c0 += 64) {
                             uint32_t v[32], o[16];
                             tmem_ld32(dx_slot + c0, v);
                             tmem_wait_ld();
@@ -748,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     if constexpr (BWD) {
-        if (warp < kSumWarp) {
+        if (warp < 8) {
             const int h = warp >> 2, w = warp & 3;
             // dw: lane = class; with 64 rows lanes 32 w + i (i < 16) hold class 16 w + i
             const int v = l.vp == 128 ? 32 * w + lane : 16 * w + lane;
@@ -777,7 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-        } else if (warp < kMmaWarp && a.bias != nullptr) {
+        } else if ((warp == kSumWarp || warp == kSumWarp + 1) && a.bias != nullptr) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 db_sh[warp - kSumWarp][64 * (q >> 1) + 2 * lane + (q & 1)] = db[q];
