@@ -408,11 +408,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         // Descriptors of 128-byte-swizzled operands, 8-row groups 1 KB apart. K-major: a K step of 16
         // is 32 bytes along the row; MN-major: 64-wide atoms 8 KB apart, a K step is 16 rows of
         // 128 bytes. The low word holds the address and the atoms' distance in 16-byte units.
-        constexpr uint32_t kHi = (1024 >> 4) | 1u << 14 | (uint32_t)kSwizzle128B << 29;
         constexpr uint32_t kAStep = A_MN ? 128 : 2, kBStep = B_MN ? 128 : 2;
-        const uint32_t lo0 = smem_u32(smem) >> 4;
-        const uint32_t a0 = lo0 | (uint32_t)(A_MN ? 8192 >> 4 : 1) << 16;
-        const uint32_t b0 = (lo0 + (kHalfBytes >> 4)) | (uint32_t)(B_MN ? 8192 >> 4 : 1) << 16;
+        const uint32_t a0 = desc_lo(smem_u32(smem), A_MN ? 8192 : 16);
+        const uint32_t b0 = desc_lo(smem_u32(smem) + kHalfBytes, B_MN ? 8192 : 16);
         int s = 0, lt = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -435,7 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 }
                 tc_fence_after();
                 const uint32_t at = s * (kStageBytes >> 4);
-                mma_pair_k4<kAStep, kBStep, kHi>(acc, a0 + at, b0 + at, idesc, kb > it.kb0);
+                mma_pair_k4<kAStep, kBStep>(acc, a0 + at, b0 + at, idesc, kb > it.kb0);
                 mma_commit_pair(&empty[s]);
                 if (++s == kStages) {
                     s = 0;

@@ -49,11 +49,9 @@ __device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t a_desc, ui
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
 }
 
-// Four K steps as one block: the descriptors' low words (address in 16-byte units, leading offset) go
-// up by a_step and b_step a step, their high words are constants. The issuing thread's own
-// instructions are what an MMA loop waits for when each step builds its descriptors (about 130
-// cycles an MMA, as long as a 256 x 256 x 16 MMA runs).
-template <uint32_t A_STEP, uint32_t B_STEP, uint32_t HI>
+// mma_ss_k4 for the pair: 256 x 256 x 16 MMAs run about 130 cycles each, which is what one took to
+// issue when every step built its descriptors.
+template <uint32_t A_STEP, uint32_t B_STEP>
 __device__ __forceinline__ void mma_pair_k4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
                                             uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -70,7 +68,7 @@ __device__ __forceinline__ void mma_pair_k4(uint32_t d_tmem, uint32_t a_lo, uint
         "add.u32 x, x, %5;\n\tadd.u32 y, y, %6;\n\t"
         "mov.b64 a, {x, %7};\n\tmov.b64 b, {y, %7};\n\t"
         "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, 1;\n\t}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP), "n"(HI)
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP), "n"(kDescHi)
         : "memory");
 }
 

@@ -192,6 +192,47 @@ __device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
 }
 
+// The high word of every 128-byte-swizzled operand descriptor with 8-row groups 1 KB apart, and the
+// low word: the address and lbo, the byte distance of the atoms along the leading dimension.
+constexpr uint32_t kDescHi = (1024 >> 4) | 1u << 14 | (uint32_t)kSwizzle128B << 29;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) {
+    return (saddr >> 4) | (lbo >> 4) << 16;
+}
+
+// One K step, and four whose descriptors' low words go up by a_step and b_step (16-byte units) a
+// step, as one block: the issuing thread's own instructions are what an MMA loop waits for when
+// each step builds its descriptors.
+__device__ __forceinline__ void mma_ss_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                          uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHi)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ss_k4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                          uint32_t a_step, uint32_t b_step, uint32_t idesc,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 a, {%1, %7};\n\tmov.b64 b, {%2, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.u32 x, %1, %5;\n\tadd.u32 y, %2, %6;\n\t"
+        "mov.b64 a, {x, %7};\n\tmov.b64 b, {y, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, x, %5;\n\tadd.u32 y, y, %6;\n\t"
+        "mov.b64 a, {x, %7};\n\tmov.b64 b, {y, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, x, %5;\n\tadd.u32 y, y, %6;\n\t"
+        "mov.b64 a, {x, %7};\n\tmov.b64 b, {y, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(a_step), "r"(b_step), "n"(kDescHi)
+        : "memory");
+}
+
 // A from tensor memory (K-major: lane = row, a 32-bit column holds two consecutive K elements).
 __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
                                        uint32_t idesc, uint32_t accumulate) {

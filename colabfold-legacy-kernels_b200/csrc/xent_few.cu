@@ -132,13 +132,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 tc_fence_after();
-                const uint32_t sw = smem_u32(smem + s * kStageBytes), sx = sw + kW;
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) {
-                    mma_ss(tmem + 64 * (t & 1), smem_desc(sw + 32 * ks, 16, 1024, kSwizzle128B),
-                           smem_desc(sx + 32 * ks, 16, 1024, kSwizzle128B), idesc,
-                           kb > 0 || ks > 0);
-                }
+                const uint32_t at = smem_u32(smem + s * kStageBytes);
+                mma_ss_k4(tmem + 64 * (t & 1), desc_lo(at, 16), desc_lo(at + kW, 16), 2, 2, idesc,
+                          kb);
                 mma_commit(&empty[s]);
             }
             if (ok) {

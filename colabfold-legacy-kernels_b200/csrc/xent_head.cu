@@ -424,29 +424,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
         } else if (warp >= kMmaWarp && lane == 0) {
-            // Descriptors are made once: a step along an operand is an addition to its address field
-            // (16-byte units). K-major: a K step of 16 columns is 32 bytes, 64 columns an atom;
-            // MN-major: a K step of 16 rows is 2 KB.
+            // Descriptors' low words, made once: a step along an operand is an addition in 16-byte
+            // units. K-major: a K step of 16 columns is 32 bytes, 64 columns an atom; MN-major: a K
+            // step of 16 rows is 2 KB.
             const uint32_t id_l = idesc_f16(E::kBf16, 128, vn, false, false);
-            const auto k_major = [](uint32_t at) { return smem_desc(at, 16, 1024, kSwizzle128B); };
-            const uint64_t w_k = k_major(smem_u32(smem));
-            const uint64_t w_n = smem_desc(smem_u32(smem), l.vp * 128, 1024, kSwizzle128B);
-            const uint64_t x_k0 = k_major(smem_u32(xs)), g_k0 = k_major(smem_u32(gs));
-            [[maybe_unused]] const uint64_t x_n0 = smem_desc(smem_u32(xs), kAtom, 1024, kSwizzle128B);
-            [[maybe_unused]] const uint64_t g_m0 = smem_desc(smem_u32(gs), kAtom, 1024, kSwizzle128B);
+            const uint32_t w_k = desc_lo(smem_u32(smem), 16);
+            const uint32_t w_n = desc_lo(smem_u32(smem), l.vp * 128);
+            const uint32_t x_k0 = desc_lo(smem_u32(xs), 16), g_k0 = desc_lo(smem_u32(gs), 16);
+            [[maybe_unused]] const uint32_t x_n0 = desc_lo(smem_u32(xs), kAtom);
+            [[maybe_unused]] const uint32_t g_m0 = desc_lo(smem_u32(gs), kAtom);
             const uint32_t w_atom = l.vp * 8, x_tile = xbytes >> 4, g_tile = gbytes >> 4;
             constexpr uint32_t kAtom16 = kAtom >> 4;
             // K-major A (atoms kAtom apart) times B, ksteps steps of K; b_step and b_atom: B's
-            // advance a step, and over the fourth. Loops of one MMA stay in the instruction cache
-            // that the workers' long code sweeps (unrolled by four: 1500 cycles where this takes X)
-            const auto product = [&](uint32_t d, uint64_t da, uint64_t dbp, uint32_t b_step,
+            // advance a step, and four
+            const auto product = [&](uint32_t d, uint32_t da, uint32_t dbp, uint32_t b_step,
                                      uint32_t b_atom, uint32_t id, int ksteps) {
+                int k = 0;
 #pragma unroll 1
-                for (int k = 0; k < ksteps; ++k) {
-                    mma_ss(d, da, dbp, id, k);
-                    const bool last = (k & 3) == 3;
-                    da += last ? kAtom16 - 6 : 2;
-                    dbp += last ? b_atom : b_step;
+                for (; k + 4 <= ksteps; k += 4) {
+                    mma_ss_k4(d, da, dbp, 2, b_step, id, k);
+                    da += kAtom16;
+                    dbp += b_atom;
+                }
+#pragma unroll 1
+                for (; k < ksteps; ++k) {
+                    mma_ss_lo(d, da, dbp, id, k);
+                    da += 2;
+                    dbp += b_step;
                 }
             };
             const auto logits = [&](int c, int slot) {
@@ -461,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return;
                 }
                 tc_fence_after();
-                product(logits_col(slot), x_k0 + b * x_tile, w_k, 2, w_atom - 6, id_l, cn >> 4);
+                product(logits_col(slot), x_k0 + b * x_tile, w_k, 2, w_atom, id_l, cn >> 4);
                 if constexpr (!BWD) {
                     mma_commit(&x_free[b]);
                 }
@@ -491,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = (base + h) & 1; ok && c < n; c += 2) {
                     const int g = base + c;
                     const auto dx_chunk = [&](int ch) {
-                        product(tmem + 128 * h, g_k0 + h * g_tile, w_n + 2 * ch * w_atom, 128, 128,
+                        product(tmem + 128 * h, g_k0 + h * g_tile, w_n + 2 * ch * w_atom, 128, 512,
                                 idesc_f16(E::kBf16, 128, min(128, cn - 128 * ch), false, true),
                                 vn >> 4);
                         mma_commit(&d_full[h]);
@@ -513,11 +517,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             break;
                         }
                     }
-                    const uint64_t dg = g_m0 + h * g_tile, dx = x_n0 + (g & nmask) * x_tile;
-#pragma unroll 1
-                    for (int ks = 0; ks < 8; ++ks) {
-                        mma_ss(dw_col, dg + 128 * ks, dx + 128 * ks, id_w, g > 0 || ks > 0);
-                    }
+                    const uint32_t dg = g_m0 + h * g_tile, dx = x_n0 + (g & nmask) * x_tile;
+                    mma_ss_k4(dw_col, dg, dx, 128, 128, id_w, g);
+                    mma_ss_k4(dw_col, dg + 512, dx + 512, 128, 128, id_w, 1);
                     mma_commit(&x_free[g & nmask]);
                     mma_commit(&dw_done[h]);
                     if (ahead) {
