@@ -1,4 +1,5 @@
-"""Build the sm_100a library: every .cu/.cpp under csrc/ into one shared object.
+"""Build the sm_100a library: every .cu/.cpp under csrc/ into one shared object, and the torch
+binding's host helper (torch_ext/tensor_table.cpp) into a Python extension beside it.
 
   python colabfold-legacy-kernels_b200/build.py [--jobs N] [--verbose]
 
@@ -18,6 +19,8 @@ CSRC = os.path.join(HERE, 'csrc')
 OUT_DIR = os.path.join(HERE, 'src', 'colabfold_legacy_kernels', 'kernels', 'sm100')
 LIB = os.path.join(OUT_DIR, 'libcflk_sm100.so')
 BUILD = os.path.join(HERE, '_build')
+TABLE_SRC = os.path.join(HERE, 'torch_ext', 'tensor_table.cpp')
+TABLE = os.path.join(OUT_DIR, '_cflk_table.so')
 
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 NVCC_FLAGS = ARCH + ['-O3', '-std=c++17', '-lineinfo', '-Xcompiler', '-fPIC',
@@ -47,13 +50,39 @@ def compile_one(src, verbose):
     return obj, r.stderr
 
 
+def build_table():
+    """The extension that reads lists of torch tensors (no run path: torch's libraries are those the
+    importing process has loaded)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    tmp = TABLE + '.tmp'
+    cmd = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden',
+           '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch._C._GLIBCXX_USE_CXX11_ABI,
+           '-I', sysconfig.get_paths()['include']]
+    for path in cpp_extension.include_paths():
+        cmd += ['-isystem', path]
+    cmd += [TABLE_SRC, '-o', tmp]
+    for path in cpp_extension.library_paths():
+        cmd += ['-L', path]
+    cmd += ['-ltorch_python', '-ltorch_cpu', '-ltorch', '-lc10']
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError('g++ failed on %s:\n%s%s' % (TABLE_SRC, r.stdout, r.stderr))
+    os.replace(tmp, TABLE)
+    return TABLE
+
+
 def build(jobs=None, verbose=False):
     """Compile and link; returns the library path. Raises on any compiler error."""
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = sources()
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs or os.cpu_count()) as ex:
+        table = ex.submit(build_table)
         results = list(ex.map(lambda s: compile_one(s, verbose), srcs))
+        table.result()
     for _, log in results:
         if verbose or 'spill' in log:
             sys.stderr.write(log)

@@ -11,8 +11,8 @@ There is no fallback: if libcflk_sm100.so is missing or cannot be loaded, every 
 """
 import ctypes
 import functools
-import operator
-from array import array
+import importlib.util
+import os
 
 import torch
 
@@ -661,30 +661,24 @@ def linear_xent_bwd(x, w, labels, lse, dloss, bias=None):
     return dx, dw, dbias
 
 
-_dtype_of = operator.attrgetter('dtype')
+_table = None
 
 
 def _tensor_table(tensors, who):
-    """Addresses, element counts and type codes of contiguous CUDA tensors, as arrays that C reads
-    in place, and their device's index. A call may hold hundreds of tensors: every step is one pass
-    of a built-in over the list."""
-    T = torch.Tensor
-    if not all(map(T.is_contiguous, tensors)):
-        raise ValueError('%s: tensors must be contiguous' % who)
+    """Addresses, element counts and type codes of contiguous CUDA tensors, as bytes that C reads
+    in place, and their device's index (torch_ext/tensor_table.cpp)."""
+    global _table
+    if _table is None:
+        path = os.path.join(os.path.dirname(library_path('attention', 100)), '_cflk_table.so')
+        spec = importlib.util.spec_from_file_location('_cflk_table', path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _table = module.tensor_table
     try:
-        codes = array('i', map(_CODES.__getitem__, map(_dtype_of, tensors)))
-    except KeyError as e:
-        raise ValueError('%s: gradients must be float16, bfloat16 or float32, got %s' %
-                         (who, e)) from None
-    devices = set(map(T.get_device, tensors))
-    if len(devices) > 1 or (devices and min(devices) < 0):
-        raise ValueError('%s: tensors must be on one CUDA device' % who)
-    return (array('q', map(T.data_ptr, tensors)), array('q', map(T.numel, tensors)), codes,
-            devices.pop() if devices else torch.cuda.current_device())
-
-
-def _at(a):
-    return a.buffer_info()[0]
+        ptrs, numel, codes, device = _table(tensors)
+    except ValueError as e:
+        raise ValueError('%s: %s' % (who, e)) from None
+    return ptrs, numel, codes, device if device >= 0 else torch.cuda.current_device()
 
 
 def grad_sumsq(grads):
@@ -694,7 +688,7 @@ def grad_sumsq(grads):
     ptrs, numel, codes, device = _tensor_table(grads, who)
     out = torch.empty(1, dtype=torch.float64, device=device)
     ws, nb = _workspace('cflk_grad_workspace_size', (len(grads),), out, who)
-    _check(lib().cflk_grad_sumsq(_stream(), len(grads), _at(ptrs), _at(numel), _at(codes),
+    _check(lib().cflk_grad_sumsq(_stream(), len(grads), ptrs, numel, codes,
                                  _ptr(out), _ptr(ws), nb), who)
     return out
 
@@ -717,7 +711,7 @@ def clip_grad_norm(grads, max_norm, *, scale=1.0, eps=1e-6, out=None, sumsq=None
     if sumsq is not None and (sumsq.dtype != torch.float64 or sumsq.numel() != 1):
         raise ValueError('grad_clip: sumsq must be one float64')
     ws, nb = _workspace('cflk_grad_workspace_size', (len(grads),), norm, who)
-    _check(lib().cflk_grad_clip(_stream(), len(grads), _at(ptrs), _at(optrs), _at(numel),
-                                _at(codes), _at(ocodes), _ptr(sumsq), float(max_norm), float(eps), float(scale),
+    _check(lib().cflk_grad_clip(_stream(), len(grads), ptrs, optrs, numel, codes, ocodes,
+                                _ptr(sumsq), float(max_norm), float(eps), float(scale),
                                 _ptr(norm), _ptr(ws), nb), who)
     return norm

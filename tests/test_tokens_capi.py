@@ -138,3 +138,27 @@ def test_sumsq_refuses():
     assert size('cflk_grad_workspace_size', -1)[0] == 1
     # more tensors than a launch takes need a sum a launch
     assert size('cflk_grad_workspace_size', 10000)[1] > size('cflk_grad_workspace_size', 1)[1]
+
+
+def test_tensor_table_reads_lists_and_refuses_what_is_no_gradient():
+    """The host helper of the torch binding, on the CPU: what it refuses, and an empty list."""
+    import importlib.util
+    import os
+
+    import torch
+
+    import colabfold_legacy_kernels as clk
+    path = os.path.join(os.path.dirname(clk.library_path('attention', 100)), '_cflk_table.so')
+    spec = importlib.util.spec_from_file_location('_cflk_table', path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    table = module.tensor_table
+    assert table([]) == (b'', b'', b'', -1) and table(()) == (b'', b'', b'', -1)
+    t = torch.zeros(4, 6)
+    for bad, why in ((t.t(), 'contiguous'), (t.double(), 'float16'), (t, 'CUDA'), (3, 'tensors'),
+                     (None, 'tensors'), (t.to_sparse(), 'contiguous'), (t[0].int(), 'float16'),
+                     (t.to('meta'), 'CUDA')):
+        with pytest.raises(ValueError, match=why):
+            table([bad])
+    with pytest.raises(TypeError):
+        table(7)
