@@ -8,7 +8,7 @@
 //
 //   * a persistent CTA an SM; it lists its labelled tokens in shared memory (blocks of 128 tokens
 //     in turn over the CTAs) and works through them 128 at a time, so positions without a label
-//     cost nothing but dx's zeros, which a warp sends as bulk copies. Where at least half of the
+//     cost nothing but dx's zeros, which two warps send as bulk copies. Where at least half of the
 //     tokens carry a label it takes whole blocks as tiles instead, x and dx as TMA boxes;
 //   * w stays in shared memory in one layout that serves as the K-major B of the logits and the
 //     N-major B of dx; a tile of x, gathered row by row by four warps' asynchronous copies, is the
@@ -50,6 +50,7 @@ constexpr int kSumWarp = 16, kMmaWarp = 18, kLoad0 = 20, kLoaders = 4;
 constexpr int kFwdSlots = 4;  // of logits in tensor memory
 constexpr int kRoundBlocks = 32;      // blocks of 128 tokens a CTA lists at a time
 constexpr int kRound = kRoundBlocks * 128;
+constexpr int kZeroRows = 8;          // rows of zeros in shared memory
 constexpr int kAtom = 128 * 128;      // 128 rows of 64 16-bit columns, 128-byte swizzle
 constexpr int kDynamicMax = 227 * 1024 - 3072;  // beside the static shared memory
 constexpr int kSms = 148;
@@ -59,7 +60,7 @@ struct Layout {
     int vp;       // rows of w in shared memory: 64 or 128
     int atoms;    // 64-column atoms of a row of x
     int nx;       // x tiles in flight (even: a warpgroup keeps its tiles)
-    int off_x, off_g, off_list, bytes;
+    int off_x, off_g, off_list, off_zero, bytes;
 };
 
 // False where the tiles do not fit shared memory or dw does not fit tensor memory.
@@ -71,13 +72,15 @@ bool make_layout(int64_t V, int64_t C, bool bwd, Layout& l) {
     l.atoms = (int)((C + 63) / 64);
     const int w = l.atoms * l.vp * 128, x = l.atoms * kAtom;
     const int g = bwd ? 2 * (l.vp / 64) * kAtom : 0;
-    const int rest = w + g + kRound * 4 + 1024;  // alignment
+    const int zero = bwd ? kZeroRows * (int)C * 2 : 0;
+    const int rest = w + g + kRound * 4 + zero + 1024;  // alignment
     for (l.nx = 4; l.nx >= 2; l.nx -= 2) {
         if (rest + l.nx * x <= kDynamicMax) {
             l.off_x = w;
             l.off_g = l.off_x + l.nx * x;
             l.off_list = l.off_g + g;
-            l.bytes = l.off_list + kRound * 4 + 1024;
+            l.off_zero = l.off_list + kRound * 4;
+            l.bytes = l.off_zero + zero + 1024;
             return true;
         }
     }
@@ -143,8 +146,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint32_t tmem_sh;
     __shared__ int abort_flag;
     __shared__ __align__(16) float bias_sh[128];
-    __shared__ __align__(16) uint4 zero_sh[32];
     __shared__ int block_count[kRoundBlocks + 1], block_list[kRoundBlocks], dense_sh, blocks_sh;
+    __shared__ unsigned labelled[4 * kRoundBlocks];  // a bit a token of the round
     __shared__ float max_sh[kThreads / 32], db_sh[2][128];
 
     const Layout& l = a.l;
@@ -165,6 +168,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         return (((long long)rd * kRoundBlocks + i) * gridDim.x + blockIdx.x) * 128 + j;
     };
 
+    // the first round's labels on their way while the CTA sets itself up
+    for (int i = warp; i < kRoundBlocks; i += kThreads / 32) {
+        const long long t = token(0, i, 4 * lane);
+        if (t < a.T) {
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(labels + t));
+        }
+    }
     if (warp == kMmaWarp) {
         if (lane == 0) {
             mbar_init(&w_full, 1);
@@ -192,8 +202,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_alloc(&tmem_sh, 512);
         tmem_relinquish();
     }
-    if (warp == kSumWarp) {
-        zero_sh[lane] = make_uint4(0, 0, 0, 0);
+    if constexpr (BWD) {
+        for (int i = threadIdx.x; i < kZeroRows * a.C / 8; i += kThreads) {
+            reinterpret_cast<uint4*>(smem + l.off_zero)[i] = make_uint4(0, 0, 0, 0);
+        }
         fence_async_smem();
     }
     if (threadIdx.x < 128) {
@@ -254,8 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true, w_ready = false;
 #pragma unroll 1
     for (int rd = 0; rd < rounds; ++rd) {
-        // list this round's tokens: the labelled ones in order from the front, the others from
-        // the back
+        // list this round's labelled tokens in order
         constexpr int kMine = (kRoundBlocks * 32 + kThreads - 1) / kThreads;  // blocks a warp
         unsigned ballots[kMine][4];
 #pragma unroll
@@ -268,6 +279,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ballots[k][j] =
                     __ballot_sync(0xffffffffu, t < a.T && label_of(labels, t, a.V) >= 0);
                 n += __popc(ballots[k][j]);
+                if (BWD && lane == 0 && i < kRoundBlocks) {
+                    labelled[4 * i + j] = ballots[k][j];
+                }
             }
             if (lane == 0 && i < kRoundBlocks) {
                 block_count[i] = n;
@@ -312,14 +326,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int before = at + __popc(ballot & ((1u << lane) - 1));
                 if ((ballot >> lane) & 1) {
                     list[before] = (int)t;
-                } else {
-                    // token 128 i + 32 j + lane of the round, `before` of them labelled
-                    const bool in = t < a.T;
-                    list[kRound - 1 - (128 * i + 32 * j + lane - before)] = in ? (int)t : -1;
-                    if (!BWD && in) {
-                        a.loss[t] = 0.f;
-                        a.lse[t] = -kInf;
-                    }
+                } else if (!BWD && t < a.T) {
+                    a.loss[t] = 0.f;
+                    a.lse[t] = -kInf;
                 }
                 at += __popc(ballot);
             }
@@ -540,22 +549,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else if (BWD && (warp == kSumWarp || warp == kSumWarp + 1)) {
-            // zeros for the rows without a label: a bulk copy of a zeroed row each
-            // (dense: of the blocks without one)
-            for (int i = threadIdx.x - 32 * kSumWarp; i < (dense ? kRound : kRound - count); i += 64) {
-                const int blk = i >> 7;
-                long long t = list[kRound - 1 - i];
-                if (dense) {
-                    t = token(rd, blk, i & 127);
-                    t = t < a.T && block_count[blk + 1] == block_count[blk] ? t : -1;
+            // zeros for the rows without a label (dense: of the blocks without one): a lane 32 tokens,
+            // each run of them as bulk copies of up to kZeroRows zeroed rows (a copy a row is what
+            // the copy engine then waits for: 114 MB in 31 us)
+            for (int w = threadIdx.x - 32 * kSumWarp; w < 4 * kRoundBlocks; w += 64) {
+                const int blk = w >> 2;
+                const long long t0 = token(rd, blk, 32 * (w & 3));
+                const long long left = a.T - t0;
+                unsigned todo = left <= 0 ? 0 : left >= 32 ? 0xffffffffu : (1u << left) - 1;
+                todo &= ~labelled[w];
+                if (dense && block_count[blk + 1] != block_count[blk]) {
+                    todo = 0;
                 }
-                if (t >= 0) {
-                    bulk_store(static_cast<T*>(a.dx) + t * a.C, smem_u32(zero_sh),
-                               a.C * 2);
+                while (todo != 0) {
+                    const int first = __ffs(todo) - 1;
+                    const unsigned rest = ~(todo >> first);  // a zero ends the run
+                    const int run = min(rest == 0 ? 32 : __ffs(rest) - 1, kZeroRows);
+                    bulk_store(static_cast<T*>(a.dx) + (t0 + first) * a.C,
+                               smem_u32(smem + l.off_zero), run * a.C * 2);
+                    todo &= ~(((1u << run) - 1) << first);
                 }
             }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            // then dbias: the columns 2 lane, 2 lane + 1 of each 64 of g, tile by tile
             const int h = warp - kSumWarp;
             for (int c = (base + h) & 1; a.bias != nullptr && c < n; c += 2) {
                 const int g = base + c;
