@@ -485,14 +485,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_after();
             };
             if constexpr (!BWD) {
-                if (warp == kMmaWarp) {
-                    for (int c = 0; ok && c < n; ++c) {
-                        const int g = base + c;
-                        if (g >= kFwdSlots) {
-                            wait(&d_free[g % kFwdSlots], g / kFwdSlots - 1);
-                        }
-                        logits(c, g % kFwdSlots);
+                // the two warps take the tiles in turn: one issues an MMA of these sizes in about 100
+                // cycles, 1650 a tile
+#pragma unroll 1
+                for (int c = (base + warp - kMmaWarp) & 1; ok && c < n; c += 2) {
+                    const int g = base + c;
+                    if (g >= kFwdSlots) {
+                        wait(&d_free[g % kFwdSlots], g / kFwdSlots - 1);
                     }
+                    logits(c, g % kFwdSlots);
                 }
             } else {
                 // This warp's tiles are those of worker group h: the logits, dx's first 128 columns
@@ -602,25 +603,53 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int h = BWD ? (warp >> 2) & 1 : warp >> 2;
             [[maybe_unused]] const int half = warp >> 3;
             const int r = ((warp & 3) << 5) | lane;        // row of the tile, tensor-memory lane
+            // a tile's row: its token, and what is loaded for it a tile ahead (without a branch round
+            // a load: the loads' latency is a quarter of a tile's time)
+            struct Row {
+                long long tok;
+                int lab;
+                bool in;
+                float lse2, dl;
+            };
+            const auto fetch = [&](int c, Row& row) {
+                const long long at = dense ? token(rd, block_list[c], r)
+                                           : (long long)list[min(c * 128 + r, count - 1)];
+                row.tok = min(at, (long long)a.T - 1);
+                row.in = dense ? at < a.T : c * 128 + r < count;
+                row.lab = label_of(labels, row.tok, a.V);
+                if constexpr (BWD) {
+                    row.lse2 = a.lse_in[row.tok];
+                    row.dl = a.dloss[row.tok];
+                }
+            };
+            constexpr int kStep = BWD ? 2 : 4;
+            int c = BWD ? (base + h) & 1 : (h - base) & 3;
+            Row next = {};
+            if (c < n) {
+                fetch(c, next);
+            }
 #pragma unroll 1
-            for (int c = BWD ? (base + h) & 1 : (h - base) & 3; c < n; c += BWD ? 2 : 4) {
+            for (; c < n; c += kStep) {
                 const int g = base + c;
                 const int sl = BWD ? h : g % kFwdSlots, turn = BWD ? g >> 1 : g / kFwdSlots;
                 const uint32_t slot = logits_col(sl) + tmem_lane_base(warp);
                 [[maybe_unused]] const uint32_t dx_slot = tmem + 128 * sl + tmem_lane_base(warp);
-                const long long at = dense ? token(rd, block_list[c], r)
-                                           : (long long)list[min(c * 128 + r, count - 1)];
-                const long long tok = min(at, (long long)a.T - 1);
-                const int lab = label_of(labels, tok, a.V);
-                const bool live = dense ? lab >= 0 && at < a.T : c * 128 + r < count;
+                const long long tok = next.tok;
+                const int lab = next.lab;
+                const bool live = next.in && lab >= 0;
                 [[maybe_unused]] GradRow grad;
                 if constexpr (BWD) {
-                    grad.lse2 = live ? a.lse_in[tok] : -kInf;
-                    grad.dl = live ? a.dloss[tok] * scale : 0.f;
+                    grad.lse2 = next.lse2;
+                    grad.dl = next.dl * scale;
                     grad.label = lab;
-                    if (grad.lse2 == -kInf) {
+                    if (!live || grad.lse2 == -kInf) {
                         grad.kill();
                     }
+                }
+                if (!BWD && c + kStep < n) {
+                    fetch(c + kStep, next);
+                }
+                if constexpr (BWD) {
                     if (a.bias != nullptr && g >= 2) {
                         // dbias has been summed from this warpgroup's last g
                         mbar_wait(&g_free[h], ((g >> 1) - 1) & 1, &g_status, kStatusSyncWait,
@@ -683,6 +712,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     fence_async_smem();
                     tc_fence_before();
                     arrive_warp(&g_full[h]);
+                    if (c + kStep < n) {
+                        fetch(c + kStep, next);
+                    }
                     // dx. Dense: into the tile of x, which its products no longer read, for the loading
                     // warp to store. Gathered: a thread stores its row, whole 32-byte sectors where
                     // the rows allow it
