@@ -759,16 +759,18 @@ __global__ void __launch_bounds__(kLocalThreads, 1)
     }
 }
 
-// The CTAs' sums in order: four channels a thread, eight threads over the CTAs.
-__global__ void __launch_bounds__(256)
+// The CTAs' sums in order: four channels a thread, kReduceSegs threads over the CTAs.
+constexpr int kReduceSegs = 16;
+
+__global__ void __launch_bounds__(32 * kReduceSegs)
     embed_local_reduce_kernel(const float4* __restrict__ partial, int parts, int total4,
                               float scale, float4* __restrict__ dtable) {
-    __shared__ float4 sh[8][32];
+    __shared__ float4 sh[kReduceSegs][32];
     const int r = threadIdx.x & 31, seg = threadIdx.x >> 5, i = blockIdx.x * 32 + r;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < total4) {
-#pragma unroll 8
-        for (int p = seg; p < parts; p += 8) {
+#pragma unroll 10
+        for (int p = seg; p < parts; p += kReduceSegs) {
             const float4 v = partial[(long long)p * total4 + i];
             s.x += v.x;
             s.y += v.y;
@@ -780,7 +782,7 @@ __global__ void __launch_bounds__(256)
     __syncthreads();
     if (seg == 0 && i < total4) {
 #pragma unroll
-        for (int k = 1; k < 8; ++k) {
+        for (int k = 1; k < kReduceSegs; ++k) {
             s.x += sh[k][r].x;
             s.y += sh[k][r].y;
             s.z += sh[k][r].z;
@@ -873,7 +875,7 @@ cudaError_t launch_embed_local(cudaStream_t s, const void* ids, const void* dout
         static_cast<const Id*>(ids), static_cast<const T*>(dout), partial, n, (int)V, (int)C,
         p.per);
     const int total4 = (int)(V * C / 4);
-    embed_local_reduce_kernel<<<(total4 + 31) / 32, 256, 0, s>>>(
+    embed_local_reduce_kernel<<<(total4 + 31) / 32, 32 * kReduceSegs, 0, s>>>(
         reinterpret_cast<const float4*>(partial), p.parts, total4, scale,
         reinterpret_cast<float4*>(dtable));
     return cudaGetLastError();

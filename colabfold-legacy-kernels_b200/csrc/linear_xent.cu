@@ -772,9 +772,9 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-constexpr int kBiasChunks = 32;
+constexpr int kBiasChunks = 256;  // at most
 
-// column sums of a piece of g: a block 256 columns of one of kBiasChunks row ranges
+// column sums of a piece of g: a block 256 columns of one of gridDim.y row ranges
 template <typename T>
 __global__ void __launch_bounds__(256)
     xent_colsum_kernel(const T* __restrict__ g, const int* __restrict__ count, int vp, int limit,
@@ -783,8 +783,8 @@ __global__ void __launch_bounds__(256)
     const int n = *count;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int col = blockIdx.x * 256 + lane * 8;
-    const int r0 = (int)((long long)n * blockIdx.y / kBiasChunks);
-    const int r1 = (int)((long long)n * (blockIdx.y + 1) / kBiasChunks);
+    const int r0 = (int)((long long)n * blockIdx.y / gridDim.y);
+    const int r1 = (int)((long long)n * (blockIdx.y + 1) / gridDim.y);
     float s[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -823,16 +823,26 @@ __global__ void __launch_bounds__(256)
     part[(long long)blockIdx.y * vp + blockIdx.x * 256 + threadIdx.x] = t;
 }
 
+// the ranges' sums in order: 32 columns a block, eight threads a column
 template <typename T>
 __global__ void __launch_bounds__(256)
-    xent_dbias_kernel(const float* __restrict__ part, int vp, int limit,
+    xent_dbias_kernel(const float* __restrict__ part, int chunks, int vp, int limit,
                       const float* __restrict__ inv, T* __restrict__ dbias) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
+    __shared__ float sh[8][32];
+    const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    float s = 0.f;
     if (c < limit) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < kBiasChunks; ++i) {
+#pragma unroll 8
+        for (int i = seg; i < chunks; i += 8) {
             s += part[(long long)i * vp + c];
+        }
+    }
+    sh[seg][lane] = s;
+    __syncthreads();
+    if (seg == 0 && c < limit) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) {
+            s += sh[k][lane];
         }
         dbias[c] = Elem<T>::from_f(s * *inv);
     }
@@ -912,13 +922,26 @@ bool make_plan(int64_t T, int64_t V, int64_t C, bool bwd, Plan& p) {
         const int64_t pieces = (tiles_v + most - 1) / most;
         p.vp = (tiles_v + pieces - 1) / pieces * PN;
         const int64_t tiles_p = p.vp / PN;
-        // K is split where the tiles leave pairs idle, into ranges of at least 8 stages
-        const auto splits = [](int64_t tiles, int64_t k) {
-            const int64_t most_k = std::max<int64_t>(1, k / (8 * PK));
-            return (int)std::max<int64_t>(1, std::min<int64_t>(most_k, kPairs / tiles));
+        // K in as many ranges as cost least: waves of tiles over the pairs, 0.4 us a 64-deep stage
+        // (a 256 x 256 tile under load), against the float32 slabs, written and read once at
+        // 6 TB/s; ranges of at least 8 stages. `direct`: one range needs no slab.
+        const auto splits = [](int64_t tiles, int64_t k, double slab_bytes, bool direct) {
+            const int64_t stages = (k + PK - 1) / PK;
+            int best = 1;
+            double least = 0;
+            for (int s = 1; s <= 64 && (s == 1 || stages / s >= 8); ++s) {
+                const double waves = (double)((tiles * s + kPairs - 1) / kPairs);
+                const double cost = waves * (double)((stages + s - 1) / s) * 0.4 +
+                                    (s == 1 && direct ? 0 : 2 * s * slab_bytes / 6e6);
+                if (s == 1 || cost < 0.98 * least) {
+                    best = s;
+                    least = cost;
+                }
+            }
+            return best;
         };
-        p.dx_splits = splits(tiles_t * tiles_c, p.vp);
-        p.dw_splits = splits(tiles_p * tiles_c, T);
+        p.dx_splits = splits(tiles_t * tiles_c, p.vp, 4.0 * p.tp * C, false);
+        p.dw_splits = splits(tiles_p * tiles_c, T, 4.0 * p.vp * C, true);
         p.g = take((size_t)p.tp * p.vp * 2);
         p.dx_acc = take((size_t)p.dx_splits * p.tp * C * 4);
         p.dw_acc = p.dw_splits > 1 ? take((size_t)p.dw_splits * p.vp * C * 4) : 0;
@@ -1102,10 +1125,13 @@ cudaError_t backward(const HeadCall& c, const Plan& p, bool& map_ok) {
         a.splits = 1;
         e = launch_gemm<T, kGrad>(c.stream, x_k, w_k, g_out, a, tiles_t * tiles_p);
         if (e == cudaSuccess && c.dbias != nullptr) {
-            xent_colsum_kernel<T><<<dim3((unsigned)tiles_p, kBiasChunks), 256, 0, c.stream>>>(
+            // eight blocks an SM, of at least 64 rows
+            const int chunks = (int)std::max<int64_t>(
+                1, std::min<int64_t>({kBiasChunks, 8 * 2 * kPairs / tiles_p, c.T / 64}));
+            xent_colsum_kernel<T><<<dim3((unsigned)tiles_p, chunks), 256, 0, c.stream>>>(
                 g, a.count, a.vp, (int)classes, db_part);
-            xent_dbias_kernel<T><<<(unsigned)tiles_p, 256, 0, c.stream>>>(
-                db_part, a.vp, (int)classes, inv, static_cast<T*>(c.dbias) + v0);
+            xent_dbias_kernel<T><<<(unsigned)((classes + 31) / 32), 256, 0, c.stream>>>(
+                db_part, chunks, a.vp, (int)classes, inv, static_cast<T*>(c.dbias) + v0);
             e = cudaGetLastError();
         }
         if (e == cudaSuccess) {

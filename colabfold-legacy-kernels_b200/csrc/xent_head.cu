@@ -845,12 +845,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// The CTAs' dw and dbias added in order: four values a thread, eight threads over the CTAs.
+// The CTAs' dw and dbias added in order: four values a thread, kSegs threads over the CTAs.
+constexpr int kSegs = 16;
+
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(32 * kSegs)
     head_reduce_kernel(const float* __restrict__ dw_part, const float* __restrict__ db_part,
                        int ctas, int V, int C, T* __restrict__ dw, T* __restrict__ dbias) {
-    __shared__ float4 sh[8][32];
+    __shared__ float4 sh[kSegs][32];
     const int r = threadIdx.x & 31, seg = threadIdx.x >> 5;
     const int total = V * C / 4;
     const int i = blockIdx.x * 32 + r;
@@ -858,8 +860,8 @@ __global__ void __launch_bounds__(256)
     if ((int)blockIdx.x < wblocks) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
         if (i < total) {
-#pragma unroll 8
-            for (int c = seg; c < ctas; c += 8) {
+#pragma unroll 10
+            for (int c = seg; c < ctas; c += kSegs) {
                 const float4 v = reinterpret_cast<const float4*>(dw_part)[(long long)c * total + i];
                 s.x += v.x;
                 s.y += v.y;
@@ -871,7 +873,7 @@ __global__ void __launch_bounds__(256)
         __syncthreads();
         if (seg == 0 && i < total) {
 #pragma unroll
-            for (int k = 1; k < 8; ++k) {
+            for (int k = 1; k < kSegs; ++k) {
                 s.x += sh[k][r].x;
                 s.y += sh[k][r].y;
                 s.z += sh[k][r].z;
@@ -884,7 +886,7 @@ __global__ void __launch_bounds__(256)
         const int v = ((int)blockIdx.x - wblocks) * 32 + r;
         float s = 0.f;
         if (v < V) {
-            for (int c = seg; c < ctas; c += 8) {
+            for (int c = seg; c < ctas; c += kSegs) {
                 s += db_part[(long long)c * V + v];
             }
         }
@@ -892,7 +894,7 @@ __global__ void __launch_bounds__(256)
         __syncthreads();
         if (seg == 0 && v < V) {
 #pragma unroll
-            for (int k = 1; k < 8; ++k) {
+            for (int k = 1; k < kSegs; ++k) {
                 s += sh[k][r].x;
             }
             dbias[v] = Elem<T>::from_f(s);
@@ -981,7 +983,7 @@ cudaError_t xent_head(const HeadCall& c, bool bwd, bool& map_ok) {
                                     : launch<T, int, true>(c, tx, tw, tdx, a);
         if (e == cudaSuccess) {
             const int blocks = (a.V * a.C / 4 + 31) / 32 + (c.bias != nullptr ? (a.V + 31) / 32 : 0);
-            head_reduce_kernel<T><<<blocks, 256, 0, c.stream>>>(
+            head_reduce_kernel<T><<<blocks, 32 * kSegs, 0, c.stream>>>(
                 a.dw_part, a.db_part, grid, a.V, a.C, static_cast<T*>(c.dw),
                 static_cast<T*>(c.dbias));
             e = cudaGetLastError();
