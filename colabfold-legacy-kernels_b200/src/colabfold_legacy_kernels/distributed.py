@@ -9,7 +9,8 @@ only exchanges are the two the path has:
     NVLink; gloo in the CPU tests);
   * the output all-gather after an inference forward, when a rank needs the whole output.
 
-The fusions need no exchange (weights are replicated, rows independent).
+The fusions need no exchange (weights are replicated, rows independent). Clipping gradients that
+are sharded over the ranks exchanges one number, the sum of squares (clip_grad_norm).
 
 The compute functions default to the B200 kernels (colabfold_legacy_kernels.b200); they are
 parameters so that the partitioning and exchange logic can be exercised on CPU ranks.
@@ -74,3 +75,20 @@ def packed_forward_gathered(p, bias, kmask, gate_bias, lims=None, *, scale, grou
                        device=out.device)
     dist.all_gather_into_tensor(full, out.contiguous(), group=group)
     return full
+
+
+def clip_grad_norm(grads, max_norm, *, group=None, sumsq=None, clip=None, **kwargs):
+    """b200.clip_grad_norm for gradients sharded over the ranks: `grads` are this rank's shards, the
+    norm is that of all ranks' together (one all-reduce of a float64 sum of squares). Gradients
+    that every rank holds whole need no group: pass them to b200.clip_grad_norm. Keyword arguments
+    as there."""
+    if sumsq is None or clip is None:
+        from . import b200
+        sumsq = sumsq or b200.grad_sumsq
+        clip = clip or b200.clip_grad_norm
+    grads = list(grads)
+    total = sumsq(grads)
+    world, _ = _world(group)
+    if world > 1:
+        dist.all_reduce(total, op=dist.ReduceOp.SUM, group=group)
+    return clip(grads, max_norm, sumsq=total, **kwargs)
