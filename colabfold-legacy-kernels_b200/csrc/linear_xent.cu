@@ -113,21 +113,26 @@ __global__ void __launch_bounds__(kPrepThreads)
     __shared__ float sm[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // labelled tokens before this block, and the largest |dloss| of all
+    // (a single block needs no counts, and finds the largest |dloss| below)
     int before = 0;
     float m = 0.f;
-    for (int i = tid; i < a.nblocks; i += kPrepThreads) {
+    for (int i = tid; a.nblocks > 1 && i < a.nblocks; i += kPrepThreads) {
         before += i < (int)blockIdx.x ? a.counts[i] : 0;
         m = fmaxf(m, a.maxs[i]);
     }
     before = warp_sum(before);
-    m = warp_max(m);
     const long long t0 = (long long)blockIdx.x * kPrepItems + tid * 4;
     int lab[4], mine = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         lab[j] = t0 + j < a.T ? label_of(labels, t0 + j, a.V) : -1;
         mine += lab[j] >= 0;
+        if (a.nblocks == 1 && a.dloss != nullptr && lab[j] >= 0) {
+            const float d = fabsf(a.dloss[t0 + j]);
+            m = d < kInf ? fmaxf(m, d) : m;
+        }
     }
+    m = warp_max(m);
     int x = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -1033,8 +1038,10 @@ cudaError_t prepare(const HeadCall& c, const Plan& p) {
     const auto run = [&](auto tag) {
         using L = decltype(tag);
         const L* labels = static_cast<const L*>(c.labels);
-        xent_count_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.stream>>>(labels, c.dloss, (int)c.T,
-                                                                     c.V, counts, maxs);
+        if (nb > 1) {
+            xent_count_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.stream>>>(
+                labels, c.dloss, (int)c.T, c.V, counts, maxs);
+        }
         xent_compact_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.stream>>>(labels, a);
     };
     if (c.labels_64) {

@@ -146,6 +146,18 @@ def test_masked_classes(V, dt, cuda_device):
     assert all((a == 0).all() for a in got[2:])
 
 
+@pytest.mark.parametrize('dt', ['bf16', 'f16'])
+def test_masked_classes_of_few_tokens(dt, cuda_device):
+    x, w, b, labels, dloss = problem(33, 900, 40, dt)
+    b[:700] = float(torch.finfo(TD[dt]).min)
+    b[100:300] = -np.inf
+    keep = np.where((labels >= 0) & (labels < 900), 700 + labels % 200, labels)
+    close(run(x, w, b, keep, dloss, dt, cuda_device), bounds(x, w, b, keep, dloss, dt))
+    got = run(x, w, np.full(900, -np.inf), labels, dloss, dt, cuda_device)
+    assert (got[0] == 0).all() and (got[1] == -np.inf).all()
+    assert all((a == 0).all() for a in got[2:])
+
+
 @pytest.mark.parametrize('V', [23, 513])
 def test_label_of_a_masked_class_and_nan(V, cuda_device):
     x, w, b, _, dloss = problem(40, V, 32, 'bf16')
