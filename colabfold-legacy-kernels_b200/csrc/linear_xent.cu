@@ -16,7 +16,7 @@
 //     log2 domain, a second kernel joins a row's pieces in order;
 //   * backward: the classes are taken in pieces; per piece the epilogue turns recomputed logits
 //     into g, rounded to the 16-bit type into the workspace, and g is multiplied by w (adding to
-//     float32 sums of dx) and, transposed, by x. The rounding of g (relative 2^-9 in bf16, 2^-12
+//     float32 sums of dx) and, transposed, by x. The rounding of g (relative 2^-8 in bf16, 2^-11
 //     in f16) is of the size of the outputs' own rounding and is what feeding the tensor cores
 //     takes; dloss is first scaled by a power of two that brings its largest magnitude to 2^13,
 //     so that f16 keeps g's small values, and the factor is taken out before the outputs round;
@@ -221,7 +221,11 @@ __global__ void __launch_bounds__(256)
 enum Kind : int { kStats = 0, kGrad = 1, kDx = 2, kDw = 3, kDwSlab = 4 };
 
 constexpr int PN = 256, PM = 256, PK = 64;  // a pair's tile, and the depth of a stage
-constexpr int kGemmThreads = 384;           // TMA warp, MMA warp, two idle, two epilogue warpgroups
+// A TMA warp, an MMA warp, two idle, and the epilogue's warpgroups, each 256 / groups columns of the
+// CTA's 128 rows. g's exponentials, roundings and stores take four, or at C = 512 the tensor cores wait
+// for them (T 4095, V 32001, forward and backward: 457 us with two, 451 with four).
+__host__ __device__ constexpr int epi_groups(int kind) { return kind == 1 ? 4 : 2; }
+__host__ __device__ constexpr int gemm_threads(int kind) { return 128 + 128 * epi_groups(kind); }
 constexpr int kEpiWarp0 = 4;
 constexpr int kStages = 5;
 constexpr int kHalfBytes = 128 * PK * 2;    // a CTA's rows of A, or of B, in a stage
@@ -349,7 +353,7 @@ private:
 };
 
 template <typename T, int KIND>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads(KIND), 1)
     xent_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                      const __grid_constant__ CUtensorMap to, const GemmArgs a) {
     using E = Elem<T>;
@@ -361,7 +365,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     __shared__ uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
     __shared__ uint32_t tmem_sh;
     __shared__ int abort_flag;
-    __shared__ __align__(16) float bias_sh[2][128];  // each warpgroup's columns of the tile
+    __shared__ __align__(16) float bias_sh[PN];  // of the tile's columns
+    constexpr int kGroups = epi_groups(KIND), kCols = PN / kGroups, kSlots = 4 / kGroups;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -375,7 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&acc_full[i], 1);
-                mbar_init(&acc_empty[i], 16);  // eight epilogue warps of each CTA
+                mbar_init(&acc_empty[i], 8 * kGroups);  // the epilogue warps of both CTAs
             }
             mbar_init(&drain, 1);
             abort_flag = 0;
@@ -484,21 +489,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         mma_commit_pair(&drain);
         mbar_wait(&drain, 0, &g_status, kStatusMmaWait, nullptr, kDrainLimitNs);
     } else if (warp >= kEpiWarp0) {
-        // epilogue: warpgroup g takes columns [128 g, 128 g + 128) of the CTA's 128 rows (thread r
-        // = row = tensor-memory lane), with its own two staging boxes, named barrier and leader
+        // epilogue: warpgroup g takes columns [kCols g, kCols (g + 1)) of the CTA's 128 rows (thread
+        // r = row = tensor-memory lane), with its own staging boxes, named barrier and leader
         const int g = (warp - kEpiWarp0) >> 2;
         const int r = ((warp & 3) << 5) | lane;
         const bool leader = lane == 0 && (warp & 3) == 0;
         const uint32_t lane_base = tmem_lane_base(warp);
-        uint8_t* slots = smem + kStages * kStageBytes + g * 2 * kBoxBytes;
+        uint8_t* slots = smem + kStages * kStageBytes + g * kSlots * kBoxBytes;
         int lt = 0, box = 0;
-        // a box of this warpgroup is free once the store of the box two before it has read it
+        // a box of this warpgroup is free once the store of the box kSlots before it has read it
         const auto next_slot = [&]() -> uint8_t* {
             if (leader) {
-                bulk_wait_read<1>();
+                bulk_wait_read<kSlots - 1>();
             }
             named_sync(1 + g, 128);
-            return slots + (box++ & 1) * kBoxBytes;
+            return slots + (box++ & (kSlots - 1)) * kBoxBytes;
         };
         [[maybe_unused]] float out_scale = 1.f;
         if constexpr (KIND == kDw) {
@@ -508,7 +513,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             const bool none = it.kb0 == it.kb1;  // an empty K range: zeros
             const int buf = lt & 1;
             const int row = it.m0 + 128 * (int)rank + r;  // of the launch's rows
-            const int col0 = it.n0 + 128 * g;
+            const int col0 = it.n0 + kCols * g;
             [[maybe_unused]] int lab = INT_MIN / 2;  // no token
             [[maybe_unused]] GradRow grad;
             grad.kill();
@@ -524,8 +529,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 }
                 if (a.bias != nullptr) {
                     named_sync(1 + g, 128);  // the previous tile's reads are done
-                    const int c = a.v0 + col0 + r;
-                    bias_sh[g][r] = c < a.V ? E::to_f(static_cast<const T*>(a.bias)[c]) : 0.f;
+                    if (r < kCols) {
+                        const int c = a.v0 + col0 + r;
+                        bias_sh[kCols * g + r] =
+                            c < a.V ? E::to_f(static_cast<const T*>(a.bias)[c]) : 0.f;
+                    }
                     named_sync(1 + g, 128);
                 }
             }
@@ -534,7 +542,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 tc_fence_after();
                 ++lt;
             }
-            const uint32_t acc = tmem + buf * PN + 128 * g + lane_base;
+            const uint32_t acc = tmem + buf * PN + kCols * g + lane_base;
             // the accumulator's 32 columns of chunk ch
             const auto load = [&](int ch, uint32_t (&v)[32]) {
                 tmem_ld32(acc + 32 * ch, v);
@@ -544,7 +552,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 // log2-domain maximum and sum of this row's columns; -inf where nothing is left
                 float m = -kInf, s = 0.f, at_label = 0.f;
                 const int limit = min(a.vp, a.V - a.v0);
-                for (int ch = 0; ch < 4; ++ch) {
+                for (int ch = 0; ch < kCols / 32; ++ch) {
                     const int c0 = col0 + 32 * ch;
                     if (c0 >= limit) {
                         break;
@@ -552,7 +560,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     uint32_t v[32];
                     load(ch, v);
                     row_stats<32>(v, c0, limit, lab,
-                                  a.bias != nullptr ? &bias_sh[g][32 * ch] : nullptr, m, s,
+                                  a.bias != nullptr ? &bias_sh[kCols * g + 32 * ch] : nullptr, m, s,
                                   at_label);
                 }
                 if (lab >= col0 && lab < min(col0 + 128, limit)) {
@@ -562,7 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 a.part[piece * a.cap + row] = make_float2(m, s);
             } else if constexpr (KIND == kGrad) {
                 const int limit = min(a.vp, a.V - a.v0);
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < kCols / 64; ++j) {
                     const int b0 = col0 + 64 * j;
                     if (b0 >= limit) {
                         break;
@@ -575,7 +583,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                         load(2 * j + h, v);
                         float y[32];
                         row_grad<32>(v, y, c0, limit, grad,
-                                 a.bias != nullptr ? &bias_sh[g][64 * j + 32 * h] : nullptr);
+                                 a.bias != nullptr ? &bias_sh[kCols * g + 64 * j + 32 * h] : nullptr);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             *reinterpret_cast<uint4*>(dst + (((4 * h + q) ^ (r & 7)) << 4)) =
@@ -593,7 +601,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     }
                 }
             } else if constexpr (KIND == kDw) {
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < kCols / 64; ++j) {
                     const int b0 = col0 + 64 * j;
                     if (b0 >= a.C) {
                         break;
@@ -630,7 +638,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     }
                 }
             } else {
-                for (int ch = 0; ch < 4; ++ch) {
+                for (int ch = 0; ch < kCols / 32; ++ch) {
                     const int c0 = col0 + 32 * ch;
                     if (c0 >= a.C) {
                         break;
@@ -1003,7 +1011,7 @@ cudaError_t launch_gemm(cudaStream_t s, const CUtensorMap& ta, const CUtensorMap
         }
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * kPairs);
-        cfg.blockDim = dim3(kGemmThreads);
+        cfg.blockDim = dim3(gemm_threads(KIND));
         cfg.dynamicSmemBytes = kSmemBytes;
         int fit = 0;
         e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg);
@@ -1012,14 +1020,14 @@ cudaError_t launch_gemm(cudaStream_t s, const CUtensorMap& ta, const CUtensorMap
         }
         fit = std::max(1, std::min(fit, kPairs));
         if (dev >= kMaxDevices) {
-            kern<<<2 * (unsigned)std::min<int64_t>(items, fit), kGemmThreads, kSmemBytes, s>>>(
+            kern<<<2 * (unsigned)std::min<int64_t>(items, fit), gemm_threads(KIND), kSmemBytes, s>>>(
                 ta, tb, to, a);
             return cudaGetLastError();
         }
         pairs[dev] = fit;
     }
     const unsigned grid = 2 * (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, pairs[dev]));
-    kern<<<grid, kGemmThreads, kSmemBytes, s>>>(ta, tb, to, a);
+    kern<<<grid, gemm_threads(KIND), kSmemBytes, s>>>(ta, tb, to, a);
     return cudaGetLastError();
 }
 
