@@ -99,6 +99,23 @@ def test_embed_bwd_many(T, V, C, cuda_device):
         assert torch.equal(got, b200().embed_bwd(tids, tdout, V))  # the same bits
 
 
+@pytest.mark.parametrize('T,V,C', [(40000, 2000, 128), (40000, 2000, 130), (6400, 3201, 128),
+                                   (6400, 3200, 128)])
+@pytest.mark.parametrize('kind', ['one', 'few', 'uniform'])
+def test_embed_bwd_rows_without_a_token_get_zeros(T, V, C, kind, cuda_device):
+    """Few tokens' rows of many: every other row has to be written all the same."""
+    rng = np.random.default_rng(V)
+    ids = make_ids(rng, T, V, 'one' if kind == 'one' else 'uniform')
+    if kind == 'few':
+        ids = np.where((ids >= 0) & (ids < V), ids // 97 * 97, ids)
+    dout = round_to(rng.standard_normal((T, C)), 'bf16')
+    # memory that held something else before
+    torch.full((V, C), 7.0, device=cuda_device)
+    got = b200().embed_bwd(torch.tensor(ids, device=cuda_device).int(),
+                           dev(dout, 'bf16', cuda_device), V, scale=0.5)
+    grad_close(ids, dout, V, 0.5, got, C)
+
+
 def test_embed_bwd_ignores_rows_without_a_token(cuda_device):
     dout = torch.full((4, 8), float('nan'), device=cuda_device)
     dout[1] = 2.0
