@@ -7,7 +7,14 @@
 // the V float32 rows it writes. The backward sorts (id, token) pairs by id (a stable radix sort:
 // the tokens of one id stay in order), cuts the sorted list into equal chunks so that an id with
 // many tokens is spread over many warps, and adds the chunks' partial sums in the order of the
-// list: no float atomics, the same bits every run.
+// list. Tables of few rows sort in shared memory instead, each CTA its own tokens. No float atomics,
+// the same bits every run; sums are float32 and round nowhere else.
+//
+// Measured: 589824 tokens, 65 rows, 128 channels, bf16: lookup 34 us (151 MB written, 4.4 TB/s;
+// a plain fill reaches 3.9, a copy 6.5), gradient 41 us (151 MB read, 3.7 TB/s). 16384 tokens,
+// 50001 rows, 1024 channels, f16: gradient 66 us, of which 205 MB of zeros and sums are about 50
+// at the fill's rate; four launches of the sort are too short to fill the machine and carry
+// most of the zeros.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -239,11 +246,11 @@ __global__ void __launch_bounds__(kSortThreads)
     }
 }
 
-// Each block puts its pairs at their places. Where the blocks are few (scanned 0) it adds the counts
-// of a digit itself, else it takes their prefix from sort_scan_kernel. Warp w owns the block's pairs [w 32 kSortRounds,
-// (w + 1) 32 kSortRounds) in rounds of 32: a pair's rank among the warp's of its digit is the
-// digit's running count plus the lower lanes of the round with the same digit, so equal digits
-// keep their order. FIRST: the pairs are (ids[t], t).
+// Each block puts its pairs at their places. Where the blocks are few (scanned 0) it adds the
+// counts of a digit itself, else it takes their prefix from sort_scan_kernel. Warp w owns the
+// block's pairs [w 32 kSortRounds, (w + 1) 32 kSortRounds) in rounds of 32: a pair's rank among the
+// warp's of its digit is the digit's running count plus the lower lanes of the round with the same
+// digit, so equal digits keep their order. FIRST: the pairs are (ids[t], t).
 template <typename Key, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads)
     sort_scatter_kernel(const Key* __restrict__ keys, const int* __restrict__ toks, int T,
@@ -452,8 +459,8 @@ __global__ void __launch_bounds__(kSumThreads)
 }
 
 // Rows that cross a chunk's end, by the chunk they begin in: its part and the following chunks' in
-// order. A warp an item (chunk, slab); rows of more than kLong parts by the block's warps together, each
-// a contiguous share of the parts.
+// order. A warp an item (chunk, slab); rows of more than kLong parts by the block's warps together,
+// each a contiguous share of the parts.
 constexpr int kLong = 9;
 
 template <int VEC>
@@ -837,6 +844,9 @@ bool plan_bwd(int64_t T, int64_t V, int64_t C, int vec, BwdPlan& p) {
         return false;
     }
     p.lanes = C <= 32 ? 8 : C <= 64 ? 16 : 32;
+    // Where a CTA's table of sums and its tokens' sort fit shared memory, us (local / sorted): T
+    // 589824, V 65, C 128 41 / 75, clipped offsets (nearly all of one row) 42 / 175; T 262144: V 23,
+    // C 256 35 / 50, V 256, C 128 25 / 39; T 512, V 23, C 256 10 / 12; T 16384, V 250, C 1024 24 / 24.
     p.local = vec >= 4 && V <= kLocalThreads && local_smem((int)V, p.lanes).bytes <= kLocalSmem;
     if (p.local) {
         p.slabs = (int)((C + 4 * p.lanes - 1) / (4 * p.lanes));

@@ -11,7 +11,7 @@
 //   * one persistent GEMM kernel serves the four products: a pair of CTAs (cta_group::2) computes
 //     256 x 256 tiles, each CTA streaming its 128 rows of A and its 128 of B by TMA through a ring
 //     of five 32 KB stages, the leader issuing the MMAs into one of two tensor-memory
-//     accumulators, two warpgroups a CTA draining the other;
+//     accumulators, two warpgroups a CTA (four where g is made) draining the other;
 //   * forward: the epilogue reduces each row's 128 columns to (max, sum of exponentials) in the
 //     log2 domain, a second kernel joins a row's pieces in order;
 //   * backward: the classes are taken in pieces; per piece the epilogue turns recomputed logits
@@ -22,7 +22,15 @@
 //     so that f16 keeps g's small values, and the factor is taken out before the outputs round;
 //   * sums, exponentials and row statistics are float32; products whose tiles are too few for the
 //     machine are split along K into float32 slabs added in order. No atomics: the same bits
-//     every run.
+//     every run;
+//   * heads of few classes (xent_head.cu) and the forward of few tokens (xent_few.cu), which HBM
+//     bounds, have kernels of their own.
+//
+// Bound by the tensor cores: 2 T V C operations forward, 6 T V C backward, 2 of them the logits
+// again, which not keeping them costs. T 4096, V 16384, C 1024, bf16, under a profiler: the logits'
+// product 96 us (tensor pipe active 82 %), g 111 (69 %), dx 101 (88 %), dw 109 (77 %). T 8192,
+// V 100003, C 2048: 13.4 TFLOP in 9.6 to 10.6 ms, 1.27 to 1.40 PFLOP/s where a library product of
+// 8192^3 holds 1.41 for seconds; the GPU's power is the limit there.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -221,9 +229,9 @@ __global__ void __launch_bounds__(256)
 enum Kind : int { kStats = 0, kGrad = 1, kDx = 2, kDw = 3, kDwSlab = 4 };
 
 constexpr int PN = 256, PM = 256, PK = 64;  // a pair's tile, and the depth of a stage
-// A TMA warp, an MMA warp, two idle, and the epilogue's warpgroups, each 256 / groups columns of the
-// CTA's 128 rows. g's exponentials, roundings and stores take four, or at C = 512 the tensor cores wait
-// for them (T 4095, V 32001, forward and backward: 457 us with two, 451 with four).
+// A TMA warp, an MMA warp, two idle, and the epilogue's warpgroups, each 256 / groups columns of
+// the CTA's 128 rows. g's exponentials, roundings and stores take four, or at C = 512 the tensor
+// cores wait for them (T 4095, V 32001, forward and backward: 457 us with two, 451 with four).
 __host__ __device__ constexpr int epi_groups(int kind) { return kind == 1 ? 4 : 2; }
 __host__ __device__ constexpr int gemm_threads(int kind) { return 128 + 128 * epi_groups(kind); }
 constexpr int kEpiWarp0 = 4;
@@ -899,7 +907,9 @@ size_t round256(size_t n) {
 
 constexpr int64_t kMax = int64_t(1) << 31;
 constexpr size_t kPartBytes = size_t(256) << 20;   // statistics pieces of one launch
-constexpr size_t kPieceBytes = size_t(512) << 20;  // g of one piece of the classes
+// g of one piece of the classes. Pieces that stay in L2 do not pay for their launches and part-
+// filled waves: T 8192, V 100003, C 2048 11.4 ms at 64 and 128 MB, 11.3 at 256, 11.1 at 512.
+constexpr size_t kPieceBytes = size_t(512) << 20;
 constexpr int kPairs = 74;
 
 struct Plan {
@@ -925,11 +935,18 @@ bool make_plan(int64_t T, int64_t V, int64_t C, bool bwd, Plan& p) {
     if (__builtin_mul_overflow(T + 256, C * 64, &mul) || __builtin_mul_overflow(V, C * 64, &mul)) {
         return false;
     }
+    // Both sides, in us (head kernels / the tiles below), forward and backward: T 589824, V 64,
+    // C 128, nine tenths labelled 37 / 172 and 83 / 615; T 262144, V 23, C 256, 15 % labelled
+    // 17 / 30 and 51 / 142, all 30 / 108 and 83 / 387; T 100000, V 128, C 128 16 / 46 and 37 / 151;
+    // T 1000, V 64, C 128 8.1 / 12.7 and 14 / 38; T 50000, V 100, C 200 14 / 32 and 110 / 108 (the
+    // widest that fit, and odd channels, break even backward).
     p.head = xent_head_fits(V, C, bwd);
     if (p.head) {
         p.bytes = xent_head_workspace(T, V, C, bwd);
         return true;
     }
+    // V 32000, C 1024, us (few / the tiles below): T 1 18 / 27, T 64 22 / 28; more tokens than one
+    // MMA's columns would read the weights twice.
     p.few = !bwd && xent_few_fits(T);
     if (p.few) {
         p.bytes = xent_few_workspace();
