@@ -24,6 +24,7 @@
 
 #include "capi_internal.h"
 #include "cflk_b200.h"
+#include "launch.cuh"
 #include "sm100.cuh"
 #include "vec_io.cuh"
 
@@ -181,6 +182,8 @@ __global__ void __launch_bounds__(kSortThreads)
     sort_count_kernel(const Key* __restrict__ keys, int T, unsigned V, int shift, int bits,
                       int* __restrict__ counts, int nblocks, uint8_t* __restrict__ mark,
                       const ZeroShare zero) {
+    wait_before();
+    begin_next();
     if ((int)blockIdx.x >= nblocks) {
         zero_rows(zero, blockIdx.x - nblocks, kSortWarps);
         return;
@@ -221,6 +224,8 @@ __global__ void __launch_bounds__(kSortThreads)
 // the sum.
 __global__ void __launch_bounds__(kSortThreads)
     sort_scan_kernel(int* __restrict__ counts, int* __restrict__ totals, int bins, int nblocks) {
+    wait_before();
+    begin_next();
     const int digit = blockIdx.x * kSortWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (digit >= bins) {
         return;
@@ -258,6 +263,8 @@ __global__ void __launch_bounds__(kSortThreads)
                         const int* __restrict__ totals, int nblocks, int scanned,
                         unsigned* __restrict__ okeys, int* __restrict__ otoks,
                         const ZeroShare zero) {
+    wait_before();
+    begin_next();
     if ((int)blockIdx.x >= nblocks) {
         zero_rows(zero, blockIdx.x - nblocks, kSortWarps);
         return;
@@ -381,6 +388,10 @@ __global__ void __launch_bounds__(kSumThreads)
                      const T* __restrict__ dout, float* __restrict__ dtable,
                      float* __restrict__ partial, int n, unsigned V, int C, int slabs, int chunks,
                      int len, int sum_blocks, float scale, const ZeroShare zero) {
+    wait_before();
+    if (chunks > 1) {
+        begin_next();
+    }
     constexpr int kUnroll = 8;
     const int lane = threadIdx.x & 31;
     const long long item = (long long)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
@@ -489,6 +500,7 @@ __global__ void __launch_bounds__(kSumThreads)
     embed_join_kernel(const unsigned* __restrict__ keys, float* __restrict__ dtable,
                       const float* __restrict__ partial, int n, unsigned V, int C, int slabs,
                       int chunks, int len, float scale) {
+    wait_before();
     __shared__ int long_last[kSumWarps];  // the last chunk of a warp's long row, or -1
     __shared__ __align__(32) float part_sum[kSumWarps][32 * VEC];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -616,6 +628,7 @@ template <typename T, typename Id, int GL>
 __global__ void __launch_bounds__(kLocalThreads, 1)
     embed_local_kernel(const Id* __restrict__ ids, const T* __restrict__ dout,
                        float* __restrict__ partial, long long n, int V, int C, long long per) {
+    begin_next();
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int kGroups = kLocalThreads / GL, kUnroll = 8;
     const LocalSmem m = local_smem(V, GL);
@@ -797,6 +810,7 @@ constexpr int kReduceSegs = 16;
 __global__ void __launch_bounds__(32 * kReduceSegs)
     embed_local_reduce_kernel(const float4* __restrict__ partial, int parts, int total4,
                               float scale, float4* __restrict__ dtable) {
+    wait_before();
     __shared__ float4 sh[kReduceSegs][32];
     const int r = threadIdx.x & 31, seg = threadIdx.x >> 5, i = blockIdx.x * 32 + r;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -910,10 +924,12 @@ cudaError_t launch_embed_local(cudaStream_t s, const void* ids, const void* dout
         static_cast<const Id*>(ids), static_cast<const T*>(dout), partial, n, (int)V, (int)C,
         p.per);
     const int total4 = (int)(V * C / 4);
-    embed_local_reduce_kernel<<<(total4 + 31) / 32, 32 * kReduceSegs, 0, s>>>(
-        reinterpret_cast<const float4*>(partial), p.parts, total4, scale,
-        reinterpret_cast<float4*>(dtable));
-    return cudaGetLastError();
+    e = cudaGetLastError();
+    return e != cudaSuccess
+               ? e
+               : launch_behind(embed_local_reduce_kernel, (total4 + 31) / 32, 32 * kReduceSegs, 0,
+                               s, reinterpret_cast<const float4*>(partial), p.parts, total4,
+                               scale, reinterpret_cast<float4*>(dtable));
 }
 
 template <typename T, typename Id>
@@ -972,23 +988,24 @@ cudaError_t launch_embed_bwd(cudaStream_t s, const void* ids, const void* dout, 
                 p.nblocks, present, ZeroShare{});
         } else {
             const ZeroShare z = next_share();
-            sort_count_kernel<unsigned><<<p.nblocks + z.blocks, kSortThreads, 0, s>>>(
-                keys[cur], (int)n, (unsigned)V, shift, p.bits, counts, p.nblocks, nullptr, z);
+            launch_behind(sort_count_kernel<unsigned>, p.nblocks + z.blocks, kSortThreads, 0, s,
+                          keys[cur], (int)n, (unsigned)V, shift, p.bits, counts, p.nblocks, nullptr,
+                          z);
         }
         const int scanned = p.nblocks > kFewBlocks;
         if (scanned) {
-            sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(
-                counts, totals, bins, p.nblocks);
+            launch_behind(sort_scan_kernel, (bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0,
+                          s, counts, totals, bins, p.nblocks);
         }
         const ZeroShare z = next_share();
         if (pass == 0) {
-            sort_scatter_kernel<Id, true><<<p.nblocks + z.blocks, kSortThreads, 0, s>>>(
-                static_cast<const Id*>(ids), nullptr, (int)n, (unsigned)V, shift, p.bits, counts,
-                totals, p.nblocks, scanned, keys[cur], toks[cur], z);
+            launch_behind(sort_scatter_kernel<Id, true>, p.nblocks + z.blocks, kSortThreads, 0, s,
+                          static_cast<const Id*>(ids), nullptr, (int)n, (unsigned)V, shift, p.bits,
+                          counts, totals, p.nblocks, scanned, keys[cur], toks[cur], z);
         } else {
-            sort_scatter_kernel<unsigned, false><<<p.nblocks + z.blocks, kSortThreads, 0, s>>>(
-                keys[cur], toks[cur], (int)n, (unsigned)V, shift, p.bits, counts, totals,
-                p.nblocks, scanned, keys[cur ^ 1], toks[cur ^ 1], z);
+            launch_behind(sort_scatter_kernel<unsigned, false>, p.nblocks + z.blocks, kSortThreads,
+                          0, s, keys[cur], toks[cur], (int)n, (unsigned)V, shift, p.bits, counts,
+                          totals, p.nblocks, scanned, keys[cur ^ 1], toks[cur ^ 1], z);
             cur ^= 1;
         }
     }
@@ -997,17 +1014,16 @@ cudaError_t launch_embed_bwd(cudaStream_t s, const void* ids, const void* dout, 
     const ZeroShare z = next_share();
     const auto sum = [&](auto tag) {
         constexpr int VEC = decltype(tag)::value;
-        embed_sum_kernel<T, VEC><<<sum_grid + z.blocks, kSumThreads, 0, s>>>(
-            keys[cur], toks[cur], static_cast<const T*>(dout), dtable, partial, (int)n,
-            (unsigned)V, (int)C, p.slabs, p.chunks, p.len, (int)sum_grid, scale, z);
+        launch_behind(embed_sum_kernel<T, VEC>, sum_grid + z.blocks, kSumThreads, 0, s, keys[cur],
+                      toks[cur], static_cast<const T*>(dout), dtable, partial, (int)n, (unsigned)V,
+                      (int)C, p.slabs, p.chunks, p.len, (int)sum_grid, scale, z);
         if (p.chunks > 1) {
             constexpr int JVEC = VEC == 1 ? 1 : 4;  // narrower slabs: more blocks for a long row
             const int slabs = (int)((C + 32 * JVEC - 1) / (32 * JVEC));
             const int64_t joins = (int64_t)p.chunks * slabs;
-            embed_join_kernel<JVEC>
-                <<<(unsigned)((joins + kSumWarps - 1) / kSumWarps), kSumThreads, 0, s>>>(
-                    keys[cur], dtable, partial, (int)n, (unsigned)V, (int)C, slabs, p.chunks,
-                    p.len, scale);
+            launch_behind(embed_join_kernel<JVEC>, (unsigned)((joins + kSumWarps - 1) / kSumWarps),
+                          kSumThreads, 0, s, keys[cur], dtable, partial, (int)n, (unsigned)V,
+                          (int)C, slabs, p.chunks, p.len, scale);
         }
     };
     if (p.vec == 8) {

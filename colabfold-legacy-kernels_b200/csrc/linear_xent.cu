@@ -41,6 +41,7 @@
 
 #include "capi_internal.h"
 #include "cflk_b200.h"
+#include "launch.cuh"
 #include "pair_mma.cuh"
 #include "sm100.cuh"
 #include "tmap.h"
@@ -62,6 +63,7 @@ template <typename L>
 __global__ void __launch_bounds__(kPrepThreads)
     xent_count_kernel(const L* __restrict__ labels, const float* __restrict__ dloss, int T,
                       long long V, int* __restrict__ counts, float* __restrict__ maxs) {
+    begin_next();
     __shared__ int sc[8];
     __shared__ float sm[8];
     int n = 0;
@@ -117,6 +119,8 @@ struct PrepArgs {
 template <typename L>
 __global__ void __launch_bounds__(kPrepThreads)
     xent_compact_kernel(const L* __restrict__ labels, const PrepArgs a) {
+    wait_before();
+    begin_next();
     __shared__ int sc[8], so[8];
     __shared__ float sm[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -199,6 +203,8 @@ __global__ void __launch_bounds__(kPrepThreads)
 __global__ void __launch_bounds__(256)
     xent_gather_kernel(const uint4* __restrict__ x, const int* __restrict__ perm,
                        const int* __restrict__ count, uint4* __restrict__ xc, int cv) {
+    wait_before();
+    begin_next();
     const int n = *count, lane = threadIdx.x & 31;
     const int end = (n + 63) & ~63;
     for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < end;
@@ -364,6 +370,8 @@ template <typename T, int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads(KIND), 1)
     xent_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                      const __grid_constant__ CUtensorMap to, const GemmArgs a) {
+    wait_before();
+    begin_next();
     using E = Elem<T>;
     constexpr bool A_MN = KIND == kDw || KIND == kDwSlab;
     constexpr bool B_MN = KIND >= kDx;
@@ -718,6 +726,7 @@ __global__ void __launch_bounds__(256)
                      const int* __restrict__ perm, const int* __restrict__ count, int row0,
                      int rows, long long cap, int pieces, float* __restrict__ loss,
                      float* __restrict__ lse) {
+    wait_before();
     __shared__ float2 sh[8][32];
     const int n = *count;
     const int r = threadIdx.x & 31, seg = threadIdx.x >> 5;
@@ -765,6 +774,7 @@ __global__ void __launch_bounds__(256)
     xent_dx_kernel(const float* __restrict__ acc, long long slab, int splits,
                    const int* __restrict__ perm, const int* __restrict__ count,
                    const float* __restrict__ inv, T* __restrict__ dx, int rows, int C) {
+    wait_before();
     const int n = *count, lane = threadIdx.x & 31;
     const float by = *inv;
     for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows;
@@ -801,6 +811,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     xent_dw_kernel(const float* __restrict__ acc, long long slab, int splits,
                    const float* __restrict__ inv, T* __restrict__ dw, long long total8) {
+    wait_before();
+    begin_next();
     const float by = *inv;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total8;
          i += (long long)gridDim.x * 256) {
@@ -829,6 +841,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     xent_colsum_kernel(const T* __restrict__ g, const int* __restrict__ count, int vp, int limit,
                        float* __restrict__ part) {
+    wait_before();
+    begin_next();
     __shared__ float sh[8][256];
     const int n = *count;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -878,6 +892,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     xent_dbias_kernel(const float* __restrict__ part, int chunks, int vp, int limit,
                       const float* __restrict__ inv, T* __restrict__ dbias) {
+    wait_before();
+    begin_next();
     __shared__ float sh[8][32];
     const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float s = 0.f;
@@ -1037,15 +1053,13 @@ cudaError_t launch_gemm(cudaStream_t s, const CUtensorMap& ta, const CUtensorMap
         }
         fit = std::max(1, std::min(fit, kPairs));
         if (dev >= kMaxDevices) {
-            kern<<<2 * (unsigned)std::min<int64_t>(items, fit), gemm_threads(KIND), kSmemBytes, s>>>(
-                ta, tb, to, a);
-            return cudaGetLastError();
+            return launch_behind(kern, 2 * (unsigned)std::min<int64_t>(items, fit),
+                                 gemm_threads(KIND), kSmemBytes, s, ta, tb, to, a);
         }
         pairs[dev] = fit;
     }
     const unsigned grid = 2 * (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, pairs[dev]));
-    kern<<<grid, gemm_threads(KIND), kSmemBytes, s>>>(ta, tb, to, a);
-    return cudaGetLastError();
+    return launch_behind(kern, grid, gemm_threads(KIND), kSmemBytes, s, ta, tb, to, a);
 }
 
 // a row-major [rows][cols] matrix in boxes of box_cols x box_rows (128-byte rows)
@@ -1096,7 +1110,12 @@ cudaError_t prepare(const HeadCall& c, const Plan& p) {
             xent_count_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.stream>>>(
                 labels, c.dloss, (int)c.T, c.V, counts, maxs);
         }
-        xent_compact_kernel<L><<<(unsigned)nb, kPrepThreads, 0, c.stream>>>(labels, a);
+        if (nb > 1) {
+            launch_behind(xent_compact_kernel<L>, (unsigned)nb, kPrepThreads, 0, c.stream, labels,
+                          a);
+        } else {
+            xent_compact_kernel<L><<<1, kPrepThreads, 0, c.stream>>>(labels, a);
+        }
     };
     if (c.labels_64) {
         run((long long)0);
@@ -1104,9 +1123,8 @@ cudaError_t prepare(const HeadCall& c, const Plan& p) {
         run(0);
     }
     const unsigned grid = (unsigned)std::min<int64_t>((c.T + 63 + 7) / 8, 148 * 8);
-    xent_gather_kernel<<<grid, 256, 0, c.stream>>>(static_cast<const uint4*>(c.x), a.perm, a.count,
-                                              reinterpret_cast<uint4*>(ws_of(c) + p.xc),
-                                              (int)(c.C / 8));
+    launch_behind(xent_gather_kernel, grid, 256, 0, c.stream, static_cast<const uint4*>(c.x),
+                  a.perm, a.count, reinterpret_cast<uint4*>(ws_of(c) + p.xc), (int)(c.C / 8));
     return cudaGetLastError();
 }
 
@@ -1137,9 +1155,9 @@ cudaError_t forward(const HeadCall& c, const Plan& p, bool& map_ok) {
         const int64_t items = (int64_t)((a.rows + PM - 1) / PM) * (a.vp / PN);
         e = launch_gemm<T, kStats>(c.stream, tx, tw, tw, a, items);
         if (e == cudaSuccess) {
-            xent_join_kernel<<<(a.rows + 31) / 32, 256, 0, c.stream>>>(
-                a.part, a.lab_logit, reinterpret_cast<int*>(ws_of(c) + p.perm), a.count, a.row0, a.rows,
-                a.cap, 2 * (a.vp / PN), c.loss, c.lse);
+            launch_behind(xent_join_kernel, (a.rows + 31) / 32, 256, 0, c.stream, a.part,
+                          a.lab_logit, reinterpret_cast<int*>(ws_of(c) + p.perm), a.count, a.row0,
+                          a.rows, a.cap, 2 * (a.vp / PN), c.loss, c.lse);
             e = cudaGetLastError();
         }
     }
@@ -1189,10 +1207,10 @@ cudaError_t backward(const HeadCall& c, const Plan& p, bool& map_ok) {
             // eight blocks an SM, of at least 64 rows
             const int chunks = (int)std::max<int64_t>(
                 1, std::min<int64_t>({kBiasChunks, 8 * 2 * kPairs / tiles_p, c.T / 64}));
-            xent_colsum_kernel<T><<<dim3((unsigned)tiles_p, chunks), 256, 0, c.stream>>>(
-                g, a.count, a.vp, (int)classes, db_part);
-            xent_dbias_kernel<T><<<(unsigned)((classes + 31) / 32), 256, 0, c.stream>>>(
-                db_part, chunks, a.vp, (int)classes, inv, static_cast<T*>(c.dbias) + v0);
+            launch_behind(xent_colsum_kernel<T>, dim3((unsigned)tiles_p, chunks), 256, 0, c.stream,
+                          g, a.count, a.vp, (int)classes, db_part);
+            launch_behind(xent_dbias_kernel<T>, (unsigned)((classes + 31) / 32), 256, 0, c.stream,
+                          db_part, chunks, a.vp, (int)classes, inv, static_cast<T*>(c.dbias) + v0);
             e = cudaGetLastError();
         }
         if (e == cudaSuccess) {
@@ -1209,18 +1227,20 @@ cudaError_t backward(const HeadCall& c, const Plan& p, bool& map_ok) {
                 e = launch_gemm<T, kDwSlab>(c.stream, g_m, x_n, dw_out, a, items);
                 if (e == cudaSuccess) {
                     const int64_t total8 = classes * c.C / 8;
-                    xent_dw_kernel<T><<<(unsigned)std::min<int64_t>((total8 + 255) / 256, 148 * 8),
-                                        256, 0, c.stream>>>(dw_acc, p.vp * c.C, a.splits, inv,
-                                                       static_cast<T*>(c.dw) + v0 * c.C, total8);
+                    launch_behind(xent_dw_kernel<T>,
+                                  (unsigned)std::min<int64_t>((total8 + 255) / 256, 148 * 8), 256,
+                                  0, c.stream, dw_acc, p.vp * c.C, a.splits, inv,
+                                  static_cast<T*>(c.dw) + v0 * c.C, total8);
                     e = cudaGetLastError();
                 }
             }
         }
     }
     if (e == cudaSuccess) {
-        xent_dx_kernel<T><<<(unsigned)std::min<int64_t>((c.T + 7) / 8, 148 * 8), 256, 0, c.stream>>>(
-            dx_acc, p.tp * c.C, p.dx_splits, reinterpret_cast<int*>(ws_of(c) + p.perm), a.count, inv,
-            static_cast<T*>(c.dx), (int)c.T, (int)c.C);
+        launch_behind(xent_dx_kernel<T>, (unsigned)std::min<int64_t>((c.T + 7) / 8, 148 * 8), 256,
+                      0, c.stream, dx_acc, p.tp * c.C, p.dx_splits,
+                      reinterpret_cast<int*>(ws_of(c) + p.perm), a.count, inv,
+                      static_cast<T*>(c.dx), (int)c.T, (int)c.C);
         e = cudaGetLastError();
     }
     return e;

@@ -22,6 +22,7 @@
 
 #include "capi_internal.h"
 #include "cflk_b200.h"
+#include "launch.cuh"
 #include "sm100.cuh"
 #include "tmap.h"
 #include "vec_io.cuh"
@@ -57,6 +58,7 @@ template <typename T, typename L>
 __global__ void __launch_bounds__(kThreads, 1)
     few_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
                const FewArgs a) {
+    begin_next();
     using E = Elem<T>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -189,6 +191,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (cls < v1) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
+                        if (j % 8 == 0 && tok0 + j >= a.T) {
+                            break;  // eights of tokens
+                        }
                         // one exponential: of the smaller of the two, relative to the larger
                         const float y = (__uint_as_float(v[j]) + bias) * kLog2e;
                         const float d = y - m[j];
@@ -209,6 +214,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             float keep_m = kLowest, keep_s = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
+                if (j % 8 == 0 && tok0 + j >= a.T) {
+                    break;
+                }
                 float top = m[j];
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) {
@@ -254,6 +262,7 @@ __global__ void __launch_bounds__(256)
     few_join_kernel(const float2* __restrict__ part, const float* __restrict__ lab_logit,
                     const L* __restrict__ labels, int T, int V, int pieces,
                     float* __restrict__ loss, float* __restrict__ lse) {
+    wait_before();
     const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (t >= T) {
         return;
@@ -343,8 +352,8 @@ cudaError_t xent_few(const HeadCall& c, bool& map_ok) {
             return e;
         }
         kern<<<grid, kThreads, kSmemBytes, c.stream>>>(tw, tx, a);
-        few_join_kernel<L><<<(a.T + 7) / 8, 256, 0, c.stream>>>(
-            a.part, a.lab_logit, static_cast<const L*>(c.labels), a.T, a.V, grid, c.loss, c.lse);
+        launch_behind(few_join_kernel<L>, (a.T + 7) / 8, 256, 0, c.stream, a.part, a.lab_logit,
+                      static_cast<const L*>(c.labels), a.T, a.V, grid, c.loss, c.lse);
         return cudaGetLastError();
     };
     if (c.labels_64) {

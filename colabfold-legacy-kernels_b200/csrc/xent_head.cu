@@ -40,6 +40,7 @@
 
 #include "capi_internal.h"
 #include "cflk_b200.h"
+#include "launch.cuh"
 #include "sm100.cuh"
 #include "tmap.h"
 #include "vec_io.cuh"
@@ -151,6 +152,9 @@ template <typename T, typename L, bool BWD>
 __global__ void __launch_bounds__(kThreads, 1)
     head_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
                 const __grid_constant__ CUtensorMap tdx, const __grid_constant__ HeadArgs a) {
+    if constexpr (BWD) {
+        begin_next();
+    }
     using E = Elem<T>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -866,6 +870,7 @@ template <typename T>
 __global__ void __launch_bounds__(32 * kSegs)
     head_reduce_kernel(const float* __restrict__ dw_part, const float* __restrict__ db_part,
                        int ctas, int V, int C, T* __restrict__ dw, T* __restrict__ dbias) {
+    wait_before();
     __shared__ float4 sh[kSegs][32];
     const int r = threadIdx.x & 31, seg = threadIdx.x >> 5;
     const int total = V * C / 4;
@@ -997,9 +1002,9 @@ cudaError_t xent_head(const HeadCall& c, bool bwd, bool& map_ok) {
                                     : launch<T, int, true>(c, tx, tw, tdx, a);
         if (e == cudaSuccess) {
             const int blocks = (a.V * a.C / 4 + 31) / 32 + (c.bias != nullptr ? (a.V + 31) / 32 : 0);
-            head_reduce_kernel<T><<<blocks, 32 * kSegs, 0, c.stream>>>(
-                a.dw_part, a.db_part, grid, a.V, a.C, static_cast<T*>(c.dw),
-                static_cast<T*>(c.dbias));
+            launch_behind(head_reduce_kernel<T>, blocks, 32 * kSegs, 0, c.stream, a.dw_part,
+                          a.db_part, grid, a.V, a.C, static_cast<T*>(c.dw),
+                          static_cast<T*>(c.dbias));
             e = cudaGetLastError();
         }
         return e;
