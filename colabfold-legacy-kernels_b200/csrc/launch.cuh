@@ -5,9 +5,10 @@
 //
 // Calls in a stream, us, so / by plain launches: gradient of 16384 tokens of 50001 rows of 1024
 // channels (six kernels) 74 / 80, cross entropy of 4095 tokens and 32001 classes and its gradients
-// (twelve) 455 / 468, of 4 tokens (two) 17.2 / 18.0. Clipping, whose second kernel finds in
-// L2 what the first one read, keeps plain launches: its blocks then stay on the SMs, and the half of
-// L2, that they had (93 M elements 147, behind one another 170).
+// (twelve) 455 / 468, of 4 tokens (two) 17.2 / 18.0. Clipping, whose second kernel finds in L2
+// what the first one read, keeps plain launches (384 tensors of 242000 float32 elements 187 / 179,
+// 300 M bf16 elements 437 / 414, 0.3 M 8.0 / 7.8): blocks that begin where others end are no
+// longer on the SM of the block that read their range.
 #pragma once
 
 #include <cuda_runtime.h>

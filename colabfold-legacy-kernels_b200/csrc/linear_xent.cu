@@ -961,7 +961,7 @@ bool make_plan(int64_t T, int64_t V, int64_t C, bool bwd, Plan& p) {
         p.bytes = xent_head_workspace(T, V, C, bwd);
         return true;
     }
-    // V 32000, C 1024, us (few / the tiles below): T 1 18 / 27, T 64 22 / 28; more tokens than one
+    // V 32000, C 1024, us (few / the tiles below): T 1 17 / 27, T 64 21 / 28; more tokens than one
     // MMA's columns would read the weights twice.
     p.few = !bwd && xent_few_fits(T);
     if (p.few) {
