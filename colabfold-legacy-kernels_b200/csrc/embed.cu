@@ -179,9 +179,8 @@ __device__ __forceinline__ bool first_of_block(unsigned* seen, unsigned key) {
 // counts[digit][block]
 template <typename Key>
 __global__ void __launch_bounds__(kSortThreads)
-    sort_count_kernel(const Key* __restrict__ keys, int T, unsigned V, int shift, int bits,
-                      int* __restrict__ counts, int nblocks, uint8_t* __restrict__ mark,
-                      const ZeroShare zero) {
+    sort_count_kernel(const Key* keys, int T, unsigned V, int shift, int bits, int* counts,
+                      int nblocks, uint8_t* mark, const ZeroShare zero) {
     wait_before();
     begin_next();
     if ((int)blockIdx.x >= nblocks) {
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(kSortThreads)
 // A warp a digit: counts[digit][*] becomes its exclusive prefix over the blocks, totals[digit]
 // the sum.
 __global__ void __launch_bounds__(kSortThreads)
-    sort_scan_kernel(int* __restrict__ counts, int* __restrict__ totals, int bins, int nblocks) {
+    sort_scan_kernel(int* counts, int* totals, int bins, int nblocks) {
     wait_before();
     begin_next();
     const int digit = blockIdx.x * kSortWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -258,11 +257,9 @@ __global__ void __launch_bounds__(kSortThreads)
 // digit, so equal digits keep their order. FIRST: the pairs are (ids[t], t).
 template <typename Key, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads)
-    sort_scatter_kernel(const Key* __restrict__ keys, const int* __restrict__ toks, int T,
-                        unsigned V, int shift, int bits, const int* __restrict__ counts,
-                        const int* __restrict__ totals, int nblocks, int scanned,
-                        unsigned* __restrict__ okeys, int* __restrict__ otoks,
-                        const ZeroShare zero) {
+    sort_scatter_kernel(const Key* keys, const int* toks, int T, unsigned V, int shift, int bits,
+                        const int* counts, const int* totals, int nblocks, int scanned,
+                        unsigned* okeys, int* otoks, const ZeroShare zero) {
     wait_before();
     begin_next();
     if ((int)blockIdx.x >= nblocks) {
@@ -384,9 +381,8 @@ constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
 // blocks past the first sum_blocks write their share of the rows without a token.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSumThreads)
-    embed_sum_kernel(const unsigned* __restrict__ keys, const int* __restrict__ toks,
-                     const T* __restrict__ dout, float* __restrict__ dtable,
-                     float* __restrict__ partial, int n, unsigned V, int C, int slabs, int chunks,
+    embed_sum_kernel(const unsigned* keys, const int* toks, const T* __restrict__ dout,
+                     float* dtable, float* partial, int n, unsigned V, int C, int slabs, int chunks,
                      int len, int sum_blocks, float scale, const ZeroShare zero) {
     wait_before();
     if (chunks > 1) {
@@ -497,9 +493,8 @@ __device__ __forceinline__ void add_parts(const float* partial, int q0, int q1, 
 
 template <int VEC>
 __global__ void __launch_bounds__(kSumThreads)
-    embed_join_kernel(const unsigned* __restrict__ keys, float* __restrict__ dtable,
-                      const float* __restrict__ partial, int n, unsigned V, int C, int slabs,
-                      int chunks, int len, float scale) {
+    embed_join_kernel(const unsigned* keys, float* dtable, const float* partial, int n, unsigned V,
+                      int C, int slabs, int chunks, int len, float scale) {
     wait_before();
     __shared__ int long_last[kSumWarps];  // the last chunk of a warp's long row, or -1
     __shared__ __align__(32) float part_sum[kSumWarps][32 * VEC];
@@ -808,8 +803,8 @@ __global__ void __launch_bounds__(kLocalThreads, 1)
 constexpr int kReduceSegs = 16;
 
 __global__ void __launch_bounds__(32 * kReduceSegs)
-    embed_local_reduce_kernel(const float4* __restrict__ partial, int parts, int total4,
-                              float scale, float4* __restrict__ dtable) {
+    embed_local_reduce_kernel(const float4* partial, int parts, int total4, float scale,
+                              float4* dtable) {
     wait_before();
     __shared__ float4 sh[kReduceSegs][32];
     const int r = threadIdx.x & 31, seg = threadIdx.x >> 5, i = blockIdx.x * 32 + r;

@@ -9,6 +9,10 @@
 // what the first one read, keeps plain launches (384 tensors of 242000 float32 elements 187 / 179,
 // 300 M bf16 elements 437 / 414, 0.3 M 8.0 / 7.8): blocks that begin where others end are no
 // longer on the SM of the block that read their range.
+//
+// Such a kernel can be at work while the one before it still writes what it will read, so only the
+// caller's own inputs are __restrict__ in it: on memory that a kernel of the call writes, that word
+// would let the compiler move accesses above wait_before or load them as data that never changes.
 #pragma once
 
 #include <cuda_runtime.h>

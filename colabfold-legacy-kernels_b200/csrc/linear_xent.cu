@@ -201,8 +201,8 @@ __global__ void __launch_bounds__(kPrepThreads)
 // xc[i] = x[perm[i]] for the labelled tokens, zeros up to the next multiple of 64 (the K slices
 // of dw read that far); a warp a row, 16 bytes a lane.
 __global__ void __launch_bounds__(256)
-    xent_gather_kernel(const uint4* __restrict__ x, const int* __restrict__ perm,
-                       const int* __restrict__ count, uint4* __restrict__ xc, int cv) {
+    xent_gather_kernel(const uint4* __restrict__ x, const int* perm, const int* count, uint4* xc,
+                       int cv) {
     wait_before();
     begin_next();
     const int n = *count, lane = threadIdx.x & 31;
@@ -722,10 +722,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads(KIND), 
 // Rows' pieces to lse and loss: 32 rows a block, eight threads a row over every eighth piece,
 // joined in order. A row with no class left (every logit -inf) counts as without a label.
 __global__ void __launch_bounds__(256)
-    xent_join_kernel(const float2* __restrict__ part, const float* __restrict__ lab_logit,
-                     const int* __restrict__ perm, const int* __restrict__ count, int row0,
-                     int rows, long long cap, int pieces, float* __restrict__ loss,
-                     float* __restrict__ lse) {
+    xent_join_kernel(const float2* part, const float* lab_logit, const int* perm, const int* count,
+                     int row0, int rows, long long cap, int pieces, float* loss, float* lse) {
     wait_before();
     __shared__ float2 sh[8][32];
     const int n = *count;
@@ -771,9 +769,8 @@ __global__ void __launch_bounds__(256)
 // others. A warp a row, eight channels a lane.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    xent_dx_kernel(const float* __restrict__ acc, long long slab, int splits,
-                   const int* __restrict__ perm, const int* __restrict__ count,
-                   const float* __restrict__ inv, T* __restrict__ dx, int rows, int C) {
+    xent_dx_kernel(const float* acc, long long slab, int splits, const int* perm, const int* count,
+                   const float* inv, T* dx, int rows, int C) {
     wait_before();
     const int n = *count, lane = threadIdx.x & 31;
     const float by = *inv;
@@ -809,8 +806,8 @@ __global__ void __launch_bounds__(256)
 // dw of a piece from its slabs, eight channels a thread
 template <typename T>
 __global__ void __launch_bounds__(256)
-    xent_dw_kernel(const float* __restrict__ acc, long long slab, int splits,
-                   const float* __restrict__ inv, T* __restrict__ dw, long long total8) {
+    xent_dw_kernel(const float* acc, long long slab, int splits, const float* inv, T* dw,
+                   long long total8) {
     wait_before();
     begin_next();
     const float by = *inv;
@@ -839,8 +836,7 @@ constexpr int kBiasChunks = 256;  // at most
 // column sums of a piece of g: a block 256 columns of one of gridDim.y row ranges
 template <typename T>
 __global__ void __launch_bounds__(256)
-    xent_colsum_kernel(const T* __restrict__ g, const int* __restrict__ count, int vp, int limit,
-                       float* __restrict__ part) {
+    xent_colsum_kernel(const T* g, const int* count, int vp, int limit, float* part) {
     wait_before();
     begin_next();
     __shared__ float sh[8][256];
@@ -890,8 +886,8 @@ __global__ void __launch_bounds__(256)
 // the ranges' sums in order: 32 columns a block, eight threads a column
 template <typename T>
 __global__ void __launch_bounds__(256)
-    xent_dbias_kernel(const float* __restrict__ part, int chunks, int vp, int limit,
-                      const float* __restrict__ inv, T* __restrict__ dbias) {
+    xent_dbias_kernel(const float* part, int chunks, int vp, int limit, const float* inv,
+                      T* dbias) {
     wait_before();
     begin_next();
     __shared__ float sh[8][32];

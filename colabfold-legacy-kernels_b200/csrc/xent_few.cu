@@ -259,9 +259,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // The CTAs' pieces of a token in order: a warp a token.
 template <typename L>
 __global__ void __launch_bounds__(256)
-    few_join_kernel(const float2* __restrict__ part, const float* __restrict__ lab_logit,
+    few_join_kernel(const float2* part, const float* lab_logit,
                     const L* __restrict__ labels, int T, int V, int pieces,
-                    float* __restrict__ loss, float* __restrict__ lse) {
+                    float* loss, float* lse) {
     wait_before();
     const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (t >= T) {

@@ -868,8 +868,8 @@ constexpr int kSegs = 16;
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kSegs)
-    head_reduce_kernel(const float* __restrict__ dw_part, const float* __restrict__ db_part,
-                       int ctas, int V, int C, T* __restrict__ dw, T* __restrict__ dbias) {
+    head_reduce_kernel(const float* dw_part, const float* db_part, int ctas, int V, int C, T* dw,
+                       T* dbias) {
     wait_before();
     __shared__ float4 sh[kSegs][32];
     const int r = threadIdx.x & 31, seg = threadIdx.x >> 5;
