@@ -705,7 +705,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_wait_ld();
                         if (dense && !live && c0 == 0 && !isfinite(__uint_as_float(v[0]))) {
                             // a row without a label may hold anything, and dw multiplies it by
-                            // zeros: NaN and infinities (which every logit shows) are cleared
+                            // its zeros of g: NaN and infinities (which every logit shows) are
+                            // cleared
 #pragma unroll 1
                             for (int p = 0; p < 8 * l.atoms; ++p) {
                                 *reinterpret_cast<uint4*>(
@@ -716,6 +717,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         float y[16];
                         row_grad<16>(v, y, c0, a.V, grad,
                                      a.bias != nullptr ? bias_sh + c0 : nullptr);
+                        if (!live) {  // zeros, whatever the logits were: a product with 0 keeps NaN
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                y[j] = 0.f;
+                            }
+                        }
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             *reinterpret_cast<uint4*>(

@@ -304,3 +304,23 @@ def test_refusals(cuda_device):
                 lambda: m.linear_xent_bwd(x, w, lab, f, f.half())):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize('dt', ['bf16', 'f16'])
+@pytest.mark.parametrize('labelled', [.6, .8, .95])
+@pytest.mark.parametrize('T,V,C', [(900, 23, 64), (900, 64, 128), (40000, 64, 128), (900, 128, 128),
+                                   (900, 100, 64), (900, 23, 256), (21000, 64, 200)])
+def test_rows_without_a_label_that_are_not_finite(T, V, C, labelled, dt, cuda_device):
+    """In rounds that take whole blocks of tokens too: rows without a label, and their dloss, reach no
+    result."""
+    for bias in (True, False):
+        x, w, b, labels, dloss = problem(T, V, C, dt, bias=bias, labelled=labelled)
+        x, out = x.copy(), np.nonzero((labels < 0) | (labels >= V))[0]
+        x[out[0::4]] = np.nan
+        x[out[1::4]] = np.inf
+        x[out[2::4]] = -np.inf
+        x[out[3::4], 5] = np.inf  # one channel
+        dloss[out] = np.nan
+        got = run(x, w, b, labels, dloss, dt, cuda_device)
+        assert all(np.isfinite(a).all() for a in (got[0], *got[2:]) if a is not None)
+        close(got, bounds(x, w, b, labels, dloss, dt))
