@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kSumThreads)
     const int c = (int)(item / slabs), slab = (int)(item - (long long)c * slabs);
     const int col = (slab * 32 + lane) * VEC;
     const bool on = col < C;
-    const int p0 = c * len, p1 = min(p0 + len, n);
+    const int p0 = c * len, p1 = n - p0 < len ? n : p0 + len;  // (p0 + len may pass 2^31)
     const unsigned prev = p0 > 0 ? keys[p0 - 1] : 0xffffffffu;
     const unsigned next = p1 < n ? keys[p1] : 0xffffffffu;
     const T* src = dout + (on ? col : 0);

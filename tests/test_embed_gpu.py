@@ -159,3 +159,16 @@ def test_refusals(cuda_device):
                 lambda: m.embed_bwd(ids, dout.double(), 3)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_embed_bwd_of_tokens_near_2_to_31(cuda_device):
+    """The last chunk of the sorted list ends less than a chunk's length below 2^31."""
+    T = 2 ** 31 - 1200
+    dout = torch.zeros(T, 1, dtype=torch.float16, device=cuda_device)
+    ids = torch.zeros(T, dtype=torch.int32, device=cuda_device)
+    ids[[3, T // 2, T - 2]] = torch.tensor([1, 2, 1], dtype=torch.int32, device=cuda_device)
+    dout[[0, 3, T // 2, T - 2, T - 1]] = torch.tensor([1., 2, 4, 8, 16], device=cuda_device).half()[:, None]
+    got = b200().embed_bwd(ids, dout, 3)
+    assert got[:, 0].tolist() == [17.0, 10.0, 4.0]
+    del dout, ids
+    torch.cuda.empty_cache()  # 47 GB with the workspace
