@@ -140,12 +140,13 @@ struct ZeroShare {
 // `block` of s.blocks, `warps` warps a block: 32 rows a block a step, its warps in turn
 __device__ __forceinline__ void zero_rows(const ZeroShare& s, int block, int warps) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int r0 = s.row0 + block * 32; r0 < s.row1; r0 += s.blocks * 32) {
-        for (int r = warp; r < min(32, s.row1 - r0); r += warps) {
+    // (a step past the last row may pass 2^31)
+    for (long long r0 = (long long)s.row0 + block * 32; r0 < s.row1; r0 += s.blocks * 32) {
+        for (int r = warp; r < min(32ll, s.row1 - r0); r += warps) {
             if (s.present[r0 + r] != 0) {
                 continue;
             }
-            float* dst = s.dtable + (long long)(r0 + r) * s.C;
+            float* dst = s.dtable + (r0 + r) * s.C;
             if (s.vec) {
                 for (int c = lane * 4; c < s.C; c += 128) {
                     *reinterpret_cast<float4*>(dst + c) = make_float4(0.f, 0.f, 0.f, 0.f);

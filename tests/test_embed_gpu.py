@@ -172,3 +172,15 @@ def test_embed_bwd_of_tokens_near_2_to_31(cuda_device):
     assert got[:, 0].tolist() == [17.0, 10.0, 4.0]
     del dout, ids
     torch.cuda.empty_cache()  # 47 GB with the workspace
+
+
+def test_embed_bwd_of_rows_near_2_to_31(cuda_device):
+    V = 2 ** 31 - 2
+    torch.full((V, 1), 7.0, device=cuda_device)  # memory that held something else before
+    ids = torch.tensor([V - 1, 0, V, V - 1, V - 40000], device=cuda_device)
+    dout = torch.tensor([1., 2, 4, 8, 16], device=cuda_device)[:, None]
+    got = b200().embed_bwd(ids, dout, V)[:, 0]
+    assert got[[0, V - 40000, V - 1]].tolist() == [2.0, 16.0, 9.0]
+    assert int(torch.count_nonzero(got)) == 3
+    del got
+    torch.cuda.empty_cache()
