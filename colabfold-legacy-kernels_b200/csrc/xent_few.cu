@@ -68,7 +68,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ int abort_flag;
     __shared__ float2 joined[8][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int v0 = blockIdx.x * a.per, v1 = min(a.V, v0 + a.per);
+    const int v0 = blockIdx.x * a.per;
+    const int v1 = a.V - v0 < a.per ? a.V : v0 + a.per;  // (v0 + per may pass 2^31)
     const int tiles = (v1 - v0 + 127) / 128, nk = (a.C + 63) / 64;
     const int cols = (a.T + 15) & ~15;
 

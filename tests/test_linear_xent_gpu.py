@@ -324,3 +324,19 @@ def test_rows_without_a_label_that_are_not_finite(T, V, C, labelled, dt, cuda_de
         got = run(x, w, b, labels, dloss, dt, cuda_device)
         assert all(np.isfinite(a).all() for a in (got[0], *got[2:]) if a is not None)
         close(got, bounds(x, w, b, labels, dloss, dt))
+
+
+def test_few_tokens_of_classes_near_2_to_31(cuda_device):
+    """Zero weights but the last class's; the tolerance is that of the losses above."""
+    V, m = 2 ** 31 - 1100, b200()
+    w = torch.zeros(V, 8, dtype=torch.bfloat16, device=cuda_device)
+    w[-1] = 1.0
+    x = torch.ones(2, 8, dtype=torch.bfloat16, device=cuda_device)
+    labels = torch.tensor([V - 1, 0], device=cuda_device)
+    loss, lse = m.linear_xent(x, w, labels)
+    z = np.log(V - 1 + np.exp(8.0))
+    assert m.device_status() == 0
+    assert (np.abs(loss.cpu().numpy() - [z - 8, z]) < 2.0 ** -16 * (1 + 2 * z)).all()
+    assert (np.abs(lse.cpu().numpy() - z * ot.LOG2E) < 2.0 ** -16 * (1 + z) * ot.LOG2E).all()
+    del w
+    torch.cuda.empty_cache()
