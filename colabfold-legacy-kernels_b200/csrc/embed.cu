@@ -857,9 +857,12 @@ bool plan_bwd(int64_t T, int64_t V, int64_t C, int vec, BwdPlan& p) {
     // Where a CTA's table of sums and its tokens' sort fit shared memory, us (local / sorted): T
     // 589824, V 65, C 128 41 / 75, clipped offsets (nearly all of one row) 42 / 175; T 262144: V 23,
     // C 256 35 / 50, V 256, C 128 25 / 39; T 512, V 23, C 256 10 / 12; T 16384, V 250, C 1024 24 / 24.
-    p.local = vec >= 4 && V <= kLocalThreads && local_smem((int)V, p.lanes).bytes <= kLocalSmem;
+    // (a grid has at most 65535 slabs)
+    const int64_t local_slabs = (C + 4 * p.lanes - 1) / (4 * p.lanes);
+    p.local = vec >= 4 && V <= kLocalThreads && local_slabs <= 65535 &&
+              local_smem((int)V, p.lanes).bytes <= kLocalSmem;
     if (p.local) {
-        p.slabs = (int)((C + 4 * p.lanes - 1) / (4 * p.lanes));
+        p.slabs = (int)local_slabs;
         // a CTA an SM, of at least 512 tokens
         const int64_t want = std::max<int64_t>(1, kSms / p.slabs);
         p.per = std::max<int64_t>(512, (T + want - 1) / want);

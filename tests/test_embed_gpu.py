@@ -184,3 +184,11 @@ def test_embed_bwd_of_rows_near_2_to_31(cuda_device):
     assert int(torch.count_nonzero(got)) == 3
     del got
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('C', [128 * 65535, 128 * 65535 + 8, 8500001])
+def test_embed_bwd_of_more_slabs_than_a_grid_has_rows(C, cuda_device):
+    dout = torch.randn(3, C, device=cuda_device)
+    ids = torch.tensor([1, -1, 1], device=cuda_device)
+    got = b200().embed_bwd(ids, dout, 2, scale=2.0)
+    assert torch.equal(got[1], 2.0 * (dout[0] + dout[2])) and (got[0] == 0).all()
