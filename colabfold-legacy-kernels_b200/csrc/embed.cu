@@ -40,20 +40,20 @@ constexpr int kFwdThreads = 256, kFwdUnroll = 4;
 
 // A thread takes kFwdUnroll vectors of VEC channels a step (their loads all in flight before the
 // first store). Rows and columns of its vectors advance by the constant stride's quotient and
-// remainder, so the loop divides nothing.
+// remainder, so the loop divides nothing. (Unsigned: a position plus a step may pass 2^31.)
 template <typename TI, typename TO, typename Id, int VEC>
 __global__ void __launch_bounds__(kFwdThreads)
     embed_kernel(const Id* __restrict__ ids, const TI* __restrict__ table, TO* __restrict__ out,
-                 long long T, long long V, int cv, float scale) {
+                 long long T, long long V, unsigned cv, float scale) {
     const long long stride = (long long)gridDim.x * kFwdThreads;
     const long long first = (long long)blockIdx.x * kFwdThreads + threadIdx.x;
     const long long drow = stride / cv;
-    const int dcol = (int)(stride - drow * cv);
+    const unsigned dcol = (unsigned)(stride - drow * cv);
     long long row = first / cv;
-    int col = (int)(first - row * cv);
+    unsigned col = (unsigned)(first - row * cv);
     while (row < T) {
         long long r[kFwdUnroll], id[kFwdUnroll];
-        int c[kFwdUnroll];
+        unsigned c[kFwdUnroll];
 #pragma unroll
         for (int u = 0; u < kFwdUnroll; ++u) {
             r[u] = row;
@@ -102,11 +102,11 @@ cudaError_t launch_embed(cudaStream_t s, const void* ids, const void* table, voi
     if (vec) {
         embed_kernel<TI, TO, Id, VEC><<<grid, kFwdThreads, 0, s>>>(
             static_cast<const Id*>(ids), static_cast<const TI*>(table), static_cast<TO*>(out), T,
-            V, (int)cv, scale);
+            V, (unsigned)cv, scale);
     } else {
         embed_kernel<TI, TO, Id, 1><<<grid, kFwdThreads, 0, s>>>(
             static_cast<const Id*>(ids), static_cast<const TI*>(table), static_cast<TO*>(out), T,
-            V, (int)cv, scale);
+            V, (unsigned)cv, scale);
     }
     return cudaGetLastError();
 }
@@ -148,11 +148,11 @@ __device__ __forceinline__ void zero_rows(const ZeroShare& s, int block, int war
             }
             float* dst = s.dtable + (r0 + r) * s.C;
             if (s.vec) {
-                for (int c = lane * 4; c < s.C; c += 128) {
+                for (unsigned c = lane * 4; c < (unsigned)s.C; c += 128) {
                     *reinterpret_cast<float4*>(dst + c) = make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             } else {
-                for (int c = lane; c < s.C; c += 32) {
+                for (unsigned c = lane; c < (unsigned)s.C; c += 32) {
                     dst[c] = 0.f;
                 }
             }
@@ -400,8 +400,8 @@ __global__ void __launch_bounds__(kSumThreads)
         return;
     }
     const int c = (int)(item / slabs), slab = (int)(item - (long long)c * slabs);
-    const int col = (slab * 32 + lane) * VEC;
-    const bool on = col < C;
+    const unsigned col = ((unsigned)slab * 32 + lane) * VEC;  // (past 2^31 in the last slab)
+    const bool on = col < (unsigned)C;
     const int p0 = c * len, p1 = n - p0 < len ? n : p0 + len;  // (p0 + len may pass 2^31)
     const unsigned prev = p0 > 0 ? keys[p0 - 1] : 0xffffffffu;
     const unsigned next = p1 < n ? keys[p1] : 0xffffffffu;
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kSumThreads)
 constexpr int kLong = 9;
 
 template <int VEC>
-__device__ __forceinline__ void add_parts(const float* partial, int q0, int q1, int C, int col,
+__device__ __forceinline__ void add_parts(const float* partial, int q0, int q1, int C, unsigned col,
                                           float (&acc)[VEC]) {
     for (int q = q0; q < q1; q += 8) {
         float v[8][VEC];
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kSumThreads)
     const long long item0 = (long long)blockIdx.x * kSumWarps;
     // (chunks fastest: the slabs of a long row fall to different blocks)
     const auto column = [&](long long item) {
-        return ((int)(item / chunks) * 32 + lane) * VEC;
+        return ((unsigned)(item / chunks) * 32 + lane) * VEC;
     };
     const long long item = item0 + warp;
     int last = -1;
@@ -526,8 +526,8 @@ __global__ void __launch_bounds__(kSumThreads)
                         break;
                     }
                 }
-                const int col = column(item);
-                if (last - c < kLong && col < C) {
+                const unsigned col = column(item);
+                if (last - c < kLong && col < (unsigned)C) {
                     float acc[VEC];
                     load_vec<float, VEC>(partial + ((long long)c * 2 + 1) * C + col, acc);
                     add_parts<VEC>(partial, c + 1, last + 1, C, col, acc);
@@ -549,8 +549,9 @@ __global__ void __launch_bounds__(kSumThreads)
         if (long_last[w] < 0) {
             continue;
         }
-        const int c = (int)((item0 + w) % chunks), col = column(item0 + w), parts = long_last[w] - c;
-        const bool on = col < C;
+        const int c = (int)((item0 + w) % chunks), parts = long_last[w] - c;
+        const unsigned col = column(item0 + w);
+        const bool on = col < (unsigned)C;
         float acc[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {

@@ -192,3 +192,15 @@ def test_embed_bwd_of_more_slabs_than_a_grid_has_rows(C, cuda_device):
     ids = torch.tensor([1, -1, 1], device=cuda_device)
     got = b200().embed_bwd(ids, dout, 2, scale=2.0)
     assert torch.equal(got[1], 2.0 * (dout[0] + dout[2])) and (got[0] == 0).all()
+
+
+@pytest.mark.parametrize('C', [2 ** 31 - 8, 2 ** 31 - 21])
+def test_channels_near_2_to_31(C, cuda_device):
+    m = b200()
+    table = torch.empty(1, C, dtype=torch.float16, device=cuda_device).uniform_(-1, 1)
+    ids = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    assert torch.equal(m.embed(ids, table), table)
+    got = m.embed_bwd(ids + 1, table, 2)  # the table as a gradient of one token
+    assert int(torch.count_nonzero(got[0])) == 0 and torch.equal(got[1], table[0].float())
+    del got, table
+    torch.cuda.empty_cache()
