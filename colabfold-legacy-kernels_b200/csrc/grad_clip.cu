@@ -320,9 +320,6 @@ int64_t fill_table(Table<N>& t, int64_t at, int64_t n, const void* const* src, v
             continue;
         }
         const int64_t c = (numel[at] + kChunk - 1) / kChunk;
-        if (t.chunks + c >= (int64_t(1) << 31)) {
-            break;
-        }
         const int i = t.n++;
         t.src[i] = src[at];
         t.dst[i] = dst != nullptr ? dst[at] : nullptr;
@@ -348,6 +345,7 @@ int check_tensors(const char* who, int64_t n, const void* const* src, void* cons
         return bad("null table");
     }
     const auto known = [](int d) { return d == kF16 || d == kBF16 || d == kF32; };
+    int64_t chunks = 0;  // a launch counts them in 32 bits, and the workspace the launches by n
     for (int64_t i = 0; i < n; ++i) {
         if (numel[i] < 0 || numel[i] >= (int64_t(1) << 44)) {
             return bad("a tensor's elements must be non-negative and below 2^44");
@@ -358,6 +356,10 @@ int check_tensors(const char* who, int64_t n, const void* const* src, void* cons
         }
         if (numel[i] == 0) {
             continue;
+        }
+        chunks += (numel[i] + kChunk - 1) / kChunk;
+        if (chunks >= (int64_t(1) << 31)) {
+            return bad("the tensors hold 2^45 elements or more together");
         }
         const size_t es = src_dtype[i] == kF32 ? 4 : 2;
         if (src[i] == nullptr || reinterpret_cast<uintptr_t>(src[i]) % es != 0) {

@@ -162,3 +162,14 @@ def test_tensor_table_reads_lists_and_refuses_what_is_no_gradient():
             table([bad])
     with pytest.raises(TypeError):
         table(7)
+
+
+def test_gradients_refuse_more_elements_than_their_workspace_counts_launches_for():
+    """A launch takes 900 tensors and below 2^31 chunks of 2^14 elements; a launch more would write past
+    the workspace."""
+    for n, one in ((4, 1 << 43), (900, 40 << 30)):
+        rc, msg = clip((256,) * n, (one,) * n, (2,) * n, (256,) * n, (2,) * n)
+        assert rc == 1 and msg.startswith('grad_clip: '), (rc, msg)
+        p, m, t = arrays((256,) * n, (one,) * n, (2,) * n)
+        rc, msg = call('cflk_grad_sumsq', Z, I64(n), p, m, t, P, P, ctypes.c_size_t(1 << 20))
+        assert rc == 1 and msg.startswith('grad_norm: '), (rc, msg)
