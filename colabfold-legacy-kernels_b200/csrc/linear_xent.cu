@@ -537,7 +537,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads(KIND), 
                 const int tok = row + (KIND == kStats ? a.row0 : 0);
                 if (tok < n) {
                     lab = a.lab[tok] - a.v0;
-                    if (KIND == kGrad && a.lse_c[tok] > -kInf) {
+                    // (a NaN lse is that of a row whose gradients are NaN in every class)
+                    if (KIND == kGrad && !(a.lse_c[tok] == -kInf)) {
                         grad.lse2 = a.lse_c[tok];
                         grad.dl = a.dl_c[tok];
                         grad.label = lab;

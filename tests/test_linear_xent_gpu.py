@@ -340,3 +340,15 @@ def test_few_tokens_of_classes_near_2_to_31(cuda_device):
     assert (np.abs(lse.cpu().numpy() - z * ot.LOG2E) < 2.0 ** -16 * (1 + z) * ot.LOG2E).all()
     del w
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('T,V', [(40, 23), (40, 513), (200, 700)])
+def test_class_that_is_nan(T, V, cuda_device):
+    """Every row's softmax is NaN then, and with it every gradient."""
+    x, w, b, labels, dloss = problem(T, V, 32, 'bf16')
+    w[7] = np.nan
+    got = run(x, w, b, labels, dloss, 'bf16', cuda_device)
+    rows = (labels >= 0) & (labels < V)
+    assert np.isnan(got[0][rows]).all() and np.isnan(got[1][rows]).all()
+    assert np.isnan(got[2][rows]).all() and (got[2][~rows] == 0).all()
+    assert np.isnan(got[3]).all() and np.isnan(got[4]).all()
