@@ -12,8 +12,8 @@
 //     256 x 256 tiles, each CTA streaming its 128 rows of A and its 128 of B by TMA through a ring
 //     of five 32 KB stages, the leader issuing the MMAs into one of two tensor-memory
 //     accumulators, two warpgroups a CTA (four where g is made) draining the other;
-//   * forward: the epilogue reduces each row's 128 columns to (max, sum of exponentials) in the
-//     log2 domain, a second kernel joins a row's pieces in order;
+//   * forward: the epilogue reduces each row's 128 columns to (max, sum of exponentials), a second
+//     kernel joins a row's pieces in order;
 //   * backward: the classes are taken in pieces; per piece the epilogue turns recomputed logits
 //     into g, rounded to the 16-bit type into the workspace, and g is multiplied by w (adding to
 //     float32 sums of dx) and, transposed, by x. The rounding of g (relative 2^-8 in bf16, 2^-11
@@ -260,7 +260,7 @@ struct GemmArgs {
     const int* lab;
     const void* bias;     // or null
     float2* part;         // kStats
-    float* lab_logit;     // natural units: a masked label's lowest value stays finite
+    float* lab_logit;
     const float* lse_c;   // kGrad
     const float* dl_c;
     const float* inv;     // kDw
@@ -566,7 +566,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads(KIND), 
                 tmem_wait_ld();
             };
             if constexpr (KIND == kStats) {
-                // log2-domain maximum and sum of this row's columns; -inf where nothing is left
+                // maximum and sum of this row's columns; -inf where nothing is left
                 float m = -kInf, s = 0.f, at_label = 0.f;
                 const int limit = min(a.vp, a.V - a.v0);
                 for (int ch = 0; ch < kCols / 32; ++ch) {
@@ -732,12 +732,7 @@ __global__ void __launch_bounds__(256)
     const int row = blockIdx.x * 32 + r;
     const bool live = row < rows && row0 + row < n;
     float m = -kInf, s = 0.f;
-    const auto join = [&](float2 p) {
-        const float m1 = fmaxf(m, p.x);
-        const float ref = m1 == -kInf ? 0.f : m1;
-        s = s * ex2(m - ref) + p.y * ex2(p.x - ref);
-        m = m1;
-    };
+    const auto join = [&](float2 p) { join_stats(m, s, p.x, p.y); };
     if (live) {
         for (int p = seg; p < pieces; p += 32) {
             float2 v[4];
@@ -759,10 +754,7 @@ __global__ void __launch_bounds__(256)
             join(sh[i][r]);
         }
         const int t = perm[row0 + row];
-        const bool none = m == -kInf && s == 0.f;
-        const float l2 = log2f(s);
-        lse[t] = none ? -kInf : m + l2;
-        loss[t] = none ? 0.f : kLn2 * (m + l2) - lab_logit[row0 + row];
+        row_loss(m, s, ref_off(m), lab_logit[row0 + row], loss[t], lse[t]);
     }
 }
 

@@ -44,8 +44,39 @@ __device__ __forceinline__ float grad_scale(float m) {
     return exp2f((float)min(14 - e, 126));
 }
 
+// What a row's exponentials are taken against in the log2 domain: its largest logit m times log2 e,
+// as a rounded product (never one fused into what it is subtracted from, so that all of a row's sums
+// mean the same value), 0 where that is -inf.
+__device__ __forceinline__ float log2_of(float m) { return __fmul_rn(m, kLog2e); }
+__device__ __forceinline__ float log2_ref(float m) {
+    const float r = log2_of(m);
+    return r == -kInf ? 0.f : r;
+}
+
+// (m, s) of a row takes another part of it in: sums s of 2^(l log2 e - log2_ref(m))
+__device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s2) {
+    const float m1 = fmaxf(m, m2), ref = log2_ref(m1);
+    s = s * ex2(log2_of(m) - ref) + s2 * ex2(log2_of(m2) - ref);
+    m = m1;
+}
+
+// A row's lse (log2 domain) and loss, from its largest logit m, the sum of 2^(l log2 e - m log2 e -
+// off) and its label's logit. The loss is their difference, which the logits' size leaves exact to a
+// rounding, and the logarithm of the sum, which is at least 1: log s + m - at_label in this order, or
+// rows that are sure of their label lose what is left of the loss to the roundings of m log2 e. No
+// loss where the lse is -inf.
+__device__ __forceinline__ void row_loss(float m, float s, float off, float at_label, float& loss,
+                                         float& lse) {
+    const bool none = log2_of(m) == -kInf && s == s;
+    const float l2 = log2f(s) + off, rest = kLn2 * l2;
+    lse = none ? -kInf : fmaf(m, kLog2e, l2);
+    loss = none ? 0.f : (m - at_label) + (rest < 0.f ? 0.f : rest);
+}
+// ... and `off` of sums against log2_ref(m)
+__device__ __forceinline__ float ref_off(float m) { return fmaf(-m, kLog2e, log2_ref(m)); }
+
 // N accumulators of a row (columns c0.. of V; `bias`, or null, their biases in shared memory, 16-byte
-// aligned) into its log2-domain maximum m and sum s (relative to m); at_label takes the label's
+// aligned) into its maximum m and sum s (relative to log2_ref(m)); at_label takes the label's
 // logit. Columns past V count as -inf; where nothing is left m stays -inf and s 0.
 template <int N>
 __device__ __forceinline__ void row_stats(const uint32_t (&v)[N], int c0, int V, int label,
@@ -85,8 +116,7 @@ __device__ __forceinline__ void row_stats(const uint32_t (&v)[N], int c0, int V,
         top = max3(top, y[j], y[j + 1]);
     }
     top = fmaxf(top, y[N - 1]);
-    const float m1 = fmaxf(m, top * kLog2e);
-    const float ref = m1 == -kInf ? 0.f : m1;
+    const float m1 = fmaxf(m, top), ref = log2_ref(m1);
     const uint64_t log2e = pk2(kLog2e, kLog2e), off = pk2(-ref, -ref);
     float part0 = 0.f, part1 = 0.f;
 #pragma unroll
@@ -95,7 +125,7 @@ __device__ __forceinline__ void row_stats(const uint32_t (&v)[N], int c0, int V,
         part0 += ex2(e.x);
         part1 += ex2(e.y);
     }
-    s = s * ex2(m - ref) + (part0 + part1);
+    s = s * ex2(log2_of(m) - ref) + (part0 + part1);
     m = m1;
 }
 

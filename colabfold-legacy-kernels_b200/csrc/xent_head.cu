@@ -689,10 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc_fence_before();
                     arrive_warp(&d_free[sl]);
                     if (live) {
-                        const bool none = m == -kInf && s == 0.f;
-                        const float l2 = log2f(s);
-                        a.lse[tok] = none ? -kInf : m + l2;
-                        a.loss[tok] = none ? 0.f : kLn2 * (m + l2) - at_label;
+                        row_loss(m, s, ref_off(m), at_label, a.loss[tok], a.lse[tok]);
                     }
                 } else {
                     uint8_t* grow = gs + h * gbytes + r * 128;

@@ -352,3 +352,30 @@ def test_class_that_is_nan(T, V, cuda_device):
     assert np.isnan(got[0][rows]).all() and np.isnan(got[1][rows]).all()
     assert np.isnan(got[2][rows]).all() and (got[2][~rows] == 0).all()
     assert np.isnan(got[3]).all() and np.isnan(got[4]).all()
+
+
+@pytest.mark.parametrize('dt', ['bf16', 'f16'])
+@pytest.mark.parametrize('T,V', [(200, 23), (200, 100), (33, 900), (200, 700), (20000, 23)])
+def test_loss_of_large_logits(T, V, dt, cuda_device):
+    """Rows of exact logits (a product each): `top` at class a, top - d at class b, 0 elsewhere. What the
+    size of the logits leaves in the loss is one rounding of top - label; the sum's at most 100
+    additions (2^-24 each), the exponentials and the logarithm (2^-22 each) stay below 2^-17."""
+    rng = np.random.default_rng(T + V)
+    C = 64
+    w = np.zeros((V, C))
+    w[np.arange(min(V, C)), np.arange(min(V, C))] = 1.0
+    top = round_to(rng.uniform(20, 2000, T), dt)
+    low = round_to(np.maximum(top - rng.choice([0, .5, 2, 20, 300], T), 0), dt)
+    a = rng.integers(0, min(V, C), T)
+    b = (a + 1 + rng.integers(0, min(V, C) - 1, T)) % min(V, C)
+    x = np.zeros((T, C))
+    x[np.arange(T), a], x[np.arange(T), b] = top, low
+    m = b200()
+    for labels in (a, b):
+        want, lse = ot.linear_xent(x, w, labels)
+        got, got_lse = m.linear_xent(dev(x, dt, cuda_device), dev(w, dt, cuda_device),
+                                     torch.tensor(labels, device=cuda_device))
+        got, got_lse = got.double().cpu().numpy(), got_lse.double().cpu().numpy()
+        assert (got >= 0).all()
+        assert (np.abs(got - want) <= 2.0 ** -17 + 2.0 ** -22 * want).all(), np.abs(got - want).max()
+        assert (np.abs(got_lse - lse) <= 2.0 ** -16 + 2.0 ** -22 * np.abs(lse)).all()
