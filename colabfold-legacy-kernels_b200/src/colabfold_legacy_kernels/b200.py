@@ -631,7 +631,8 @@ def _xent_sizes(x, w, labels, bias, who):
 def linear_xent(x, w, labels, bias=None):
     """Softmax cross entropy of the classes x w^T + bias without keeping them: (loss, lse), both
     float32 of labels' shape, lse in the log2 domain. x [...,C], w [V,C], labels int32 or int64
-    [...]; a label outside [0, V) gives loss 0 and lse -inf."""
+    [...]; a label outside [0, V), or a row whose every class is masked (by -inf or by bfloat16's
+    lowest value), gives loss 0 and lse -inf."""
     who = 'linear_xent'
     dt, l64, T, V, C = _xent_sizes(x, w, labels, bias, who)
     ws, n = _workspace('cflk_linear_xent_workspace_size', (T, V, C), x, who)

@@ -292,9 +292,10 @@ CFLK_API int cflk_embed_bwd(void* stream, int dtype, int ids_64, const void* ids
  * log(sum_v exp l[t,v]) - l[t, labels[t]] and, in the log2 domain as the attention's, lse[t] =
  * log2(sum_v exp l[t,v]). x [T,C], w [V,C] 16-bit, bias [V] 16-bit or NULL, loss and lse [T]
  * float32. A token whose label is outside [0, V) gets loss 0 and lse -inf and its row of x is not
- * used (it may hold NaN); so does one whose every logit is -inf. C a multiple of 8, any V >= 1;
- * x and w 16-byte aligned. Products accumulate in float32 (tcgen05). workspace: at least the size
- * function's bytes, 256-byte aligned. */
+ * used (it may hold NaN). Loss 0 and lse -inf also where no class is left: every logit is -inf, or so
+ * low (below -2.3587e38, as bf16's lowest value as a mask makes it) that the lse leaves float32; the
+ * gradients of such a row are zero. C a multiple of 8, any V >= 1; x and w 16-byte aligned. Products
+ * accumulate in float32 (tcgen05). workspace: at least the size function's bytes, 256-byte aligned. */
 CFLK_API int cflk_linear_xent_workspace_size(int64_t T, int64_t V, int64_t C, size_t* bytes);
 CFLK_API int cflk_linear_xent(void* stream, int dtype, int labels_64, const void* x,
                               const void* w, const void* bias, const void* labels, float* loss,
@@ -304,7 +305,7 @@ CFLK_API int cflk_linear_xent(void* stream, int dtype, int labels_64, const void
 /* The gradients of cflk_linear_xent for dloss [T] float32 and the forward's lse: with g[t,v] =
  * dloss[t] (exp(l[t,v]) / sum - [v = labels[t]]), dx [T,C] = g w, dw [V,C] = g^T x and dbias [V]
  * = sum_t g (16-bit; dbias NULL exactly when bias is). Every row is written: dx is zero for tokens
- * without a label and for those whose lse is -inf. The logits are computed again, in pieces of
+ * without a label and for those whose lse is -inf (no class left). The logits are computed again, in pieces of
  * the classes, and g is rounded to the 16-bit type between the products (scaled by a power of
  * two first, so that float16 keeps its small values); sums are float32 in a fixed order. x, w, dx
  * and dw 16-byte aligned; workspace as above. */

@@ -7,6 +7,7 @@ include/cflk_b200.h.
 import numpy as np
 
 LOG2E = 1.0 / np.log(2.0)
+F32_MAX = float(np.finfo(np.float32).max)
 
 
 def embed(ids, table, scale):
@@ -37,7 +38,8 @@ def _labelled(x, w, labels, bias):
         if bias is not None:
             logits = logits + np.asarray(bias, np.float64)
     top = logits.max(1, initial=-np.inf)
-    left = top > -np.inf  # rows with a class left
+    # rows with a class left: their lse is float32 in the log2 domain
+    left = ~(top * LOG2E < -F32_MAX)
     return rows[left], labels[rows[left]], logits[left], top[left]
 
 

@@ -379,3 +379,18 @@ def test_loss_of_large_logits(T, V, dt, cuda_device):
         assert (got >= 0).all()
         assert (np.abs(got - want) <= 2.0 ** -17 + 2.0 ** -22 * want).all(), np.abs(got - want).max()
         assert (np.abs(got_lse - lse) <= 2.0 ** -16 + 2.0 ** -22 * np.abs(lse)).all()
+
+
+@pytest.mark.parametrize('T,V', [(150, 23), (33, 900), (150, 300), (150, 700)])
+def test_every_class_at_bf16s_lowest_value(T, V, cuda_device):
+    """Logits below -2.3e38 leave float32 in the log2 domain: they count as -inf, in both directions."""
+    x, w, b, labels, dloss = problem(T, V, 32, 'bf16')
+    lowest = float(torch.finfo(torch.bfloat16).min)
+    got = run(x, w, np.full(V, lowest), labels, dloss, 'bf16', cuda_device)
+    assert (got[0] == 0).all() and (got[1] == -np.inf).all()
+    assert all((a == 0).all() for a in got[2:])
+    # one class above it takes every row
+    b = np.full(V, lowest)
+    b[V - 2] = 1.0
+    keep = np.where((labels >= 0) & (labels < V), V - 2, labels)
+    close(run(x, w, b, keep, dloss, 'bf16', cuda_device), bounds(x, w, b, keep, dloss, 'bf16'))
