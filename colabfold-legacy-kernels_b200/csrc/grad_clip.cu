@@ -6,11 +6,12 @@
 // `scale` takes a loss scale out. Bound by HBM: every gradient is read once for the norm, read
 // again (out of L2 where all of them fit) and written once for the clip. Two launches: the first
 // leaves one float64 sum a block, the second adds those in a fixed order in every block (about
-// 9 KB out of L2) and scales. Neither has atomics, so a call's bits depend on its sizes and
-// values only. Tensors are cut into chunks of kChunk elements and the blocks take equal ranges of
-// them, so a thousand small tensors and one large one spread alike; the table of tensors travels as a kernel
-// parameter (no copy, nothing to keep alive on the host), kTable tensors a launch. A block's
-// clip goes backwards through the chunks: it finds what its norm read last still in L2.
+// 9 KB out of L2) and scales. Neither has atomics, so a call's bits depend on its tensors' sizes,
+// alignment and values only. Tensors are cut into chunks of kChunk elements and the blocks take
+// equal ranges of them, so a thousand small tensors and one large one spread alike; the table of
+// tensors travels as a kernel parameter (no copy, nothing to keep alive on the host), kTable tensors
+// a launch. A block's clip goes backwards through the chunks: it finds what its norm read last still
+// in L2.
 //
 // 300 M bf16 elements clipped into float32: norm 114 us (5.3 TB/s), clip 318 us (600 MB read, 1.2 GB
 // written, 5.7 TB/s). 93 M elements in 384 tensors, half of them 16-bit, in place: 58 and 93 us.
@@ -92,9 +93,9 @@ __device__ __forceinline__ double block_sum(double x) {
     return s;
 }
 
-// The sum of a vector's squares: in float32 (three roundings at most, 16-bit types' squares are
-// exact), then widened, one conversion for 4 or 8 elements: a conversion each would bound the
-// kernel (300 M bf16 elements 132 us, so 114). A sum that left float32's normal range is taken again in
+// The sum of a vector's squares: in float32 (three roundings at most on a square's way, 3 2^-24
+// relative; bf16's and f16's squares are exact), then widened, one conversion for 4 or 8 elements: a
+// conversion each would bound the kernel (300 M bf16 elements 132 us, so 114). A sum that left float32's normal range is taken again in
 // float64: squares overflow float32 from 2^64 on and lose bits below 2^-63.
 template <typename T>
 __device__ __forceinline__ double vector_sumsq(const Raw<T, 16 / (int)sizeof(T)>& r) {

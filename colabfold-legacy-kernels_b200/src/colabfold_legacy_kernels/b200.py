@@ -683,7 +683,8 @@ def _tensor_table(tensors, who):
 
 
 def grad_sumsq(grads):
-    """The sum of the squares of all elements of the tensors: float64 [1] on their device."""
+    """The sum of the squares of all elements of the tensors: float64 [1] on their device. Squares are
+    added in float32 over 16 bytes (3 2^-24 relative at most) and in float64 beyond."""
     who = 'grad_norm'
     grads = list(grads)
     ptrs, numel, codes, device = _tensor_table(grads, who)

@@ -321,8 +321,10 @@ CFLK_API int cflk_linear_xent_bwd(void* stream, int dtype, int labels_64, const 
  * alignment its type allows (below 2^44 elements a tensor, 2^45 together). workspace: at least cflk_grad_workspace_size(n) bytes, 8-byte
  * aligned; its contents do not matter.
  *
- * cflk_grad_sumsq: *sumsq (device, float64) = the sum of the squares of all elements, taken and
- * added in float64. */
+ * cflk_grad_sumsq: *sumsq (device, float64) = the sum of the squares of all elements. Those of an
+ * aligned 16-byte vector (8 or 4 elements) are added in float32, within 3 2^-24 relative, or in
+ * float64 where they leave its range; everything else is float64, in an order that the tensors'
+ * sizes and alignment fix. */
 CFLK_API int cflk_grad_workspace_size(int64_t n, size_t* bytes);
 CFLK_API int cflk_grad_sumsq(void* stream, int64_t n, const void* const* grads,
                              const int64_t* numel, const int* dtypes, double* sumsq,

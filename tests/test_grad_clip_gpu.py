@@ -153,3 +153,17 @@ def test_refusals(cuda_device):
         with pytest.raises(ValueError):
             bad()
     assert (g == 1).all()
+
+
+def test_sum_of_squares_of_few_elements(cuda_device):
+    """The squares of 16 bytes of float32 are added in float32: three roundings, 3 2^-24 relative; of 16-bit
+    types they are exact and added in three; all else is float64 (2^-50 here)."""
+    m = b200()
+    rng = np.random.default_rng(2)
+    for kind in ('f32', 'bf16', 'f16'):
+        for n in (4, 8, 12, 40, 9):
+            for _ in range(40):
+                a = round_to(rng.uniform(.5, 2, n), kind)
+                t = torch.tensor(np.asarray(a, np.float32), device=cuda_device).to(TD[kind])
+                want = float((a.astype(np.float64) ** 2).sum())
+                assert abs(m.grad_sumsq([t]).item() - want) <= (3 * 2.0 ** -24 + 2.0 ** -50) * want
