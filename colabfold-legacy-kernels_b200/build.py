@@ -1,5 +1,6 @@
-"""Build the sm_100a library: every .cu/.cpp under csrc/ into one shared object, and the torch
-binding's host helper (torch_ext/tensor_table.cpp) into a Python extension beside it.
+"""Build the sm_100a library: every .cu/.cpp under csrc/ into one shared object, and, where torch is
+installed, the torch binding's host helper (torch_ext/tensor_table.cpp) into a Python extension
+beside it.
 
   python colabfold-legacy-kernels_b200/build.py [--jobs N] [--verbose]
 
@@ -52,10 +53,13 @@ def compile_one(src, verbose):
 
 def build_table():
     """The extension that reads lists of torch tensors (no run path: torch's libraries are those the
-    importing process has loaded)."""
+    importing process has loaded). None where torch is not installed: only the torch binding wants it."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        return None
     from torch.utils import cpp_extension
     tmp = TABLE + '.tmp'
     cmd = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden',
@@ -75,14 +79,14 @@ def build_table():
 
 
 def build(jobs=None, verbose=False):
-    """Compile and link; returns the library path. Raises on any compiler error."""
+    """Compile and link; returns the library path. Raises on any compiler error; one in the torch
+    binding's helper only after the library is linked."""
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = sources()
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs or os.cpu_count()) as ex:
         table = ex.submit(build_table)
         results = list(ex.map(lambda s: compile_one(s, verbose), srcs))
-        table.result()
     for _, log in results:
         if verbose or 'spill' in log:
             sys.stderr.write(log)
@@ -94,6 +98,7 @@ def build(jobs=None, verbose=False):
     if r.returncode != 0:
         raise RuntimeError('link failed:\n%s%s' % (r.stdout, r.stderr))
     os.replace(tmp, LIB)
+    table.result()
     return LIB
 
 

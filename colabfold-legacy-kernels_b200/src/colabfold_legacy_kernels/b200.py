@@ -671,9 +671,13 @@ def _tensor_table(tensors, who):
     global _table
     if _table is None:
         path = os.path.join(os.path.dirname(library_path('attention', 100)), '_cflk_table.so')
-        spec = importlib.util.spec_from_file_location('_cflk_table', path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        try:
+            spec = importlib.util.spec_from_file_location('_cflk_table', path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise RuntimeError('%s: %s cannot be loaded: build the library with this torch installed '
+                               '(%s)' % (who, path, e)) from None
         _table = module.tensor_table
     try:
         ptrs, numel, codes, device = _table(tensors)
