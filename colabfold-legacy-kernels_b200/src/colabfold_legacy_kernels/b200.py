@@ -593,13 +593,16 @@ def embed(ids, table, *, scale=1.0, out_dtype=None, out=None):
         raise ValueError('embed: table must be [V,C]')
     V, C = table.shape
     i64 = _index_64(ids, 'ids', who)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((*ids.shape, C), dtype=out_dtype or table.dtype, device=table.device)
     if out.numel() != ids.numel() * C or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError('embed: out must be [*ids.shape, C] of out_dtype')
     rc = lib().cflk_embed(_stream(), _code(table, 'table', who), _code(out, 'out', who), i64,
                           _ptr(ids), _ptr(table), _ptr(out), ids.numel(), V, C, float(scale))
     _check(rc, who)
+    if given and not out.is_inference():
+        torch.autograd.graph.increment_version(out)  # as torch's own in-place operators do
     return out
 
 
@@ -665,9 +668,8 @@ def linear_xent_bwd(x, w, labels, lse, dloss, bias=None):
 _table = None
 
 
-def _tensor_table(tensors, who):
-    """Addresses, element counts and type codes of contiguous CUDA tensors, as bytes that C reads
-    in place, and their device's index (torch_ext/tensor_table.cpp)."""
+def _helper(who):
+    """The module built from torch_ext/tensor_table.cpp."""
     global _table
     if _table is None:
         path = os.path.join(os.path.dirname(library_path('attention', 100)), '_cflk_table.so')
@@ -678,9 +680,15 @@ def _tensor_table(tensors, who):
         except ImportError as e:
             raise RuntimeError('%s: %s cannot be loaded: build the library with this torch installed '
                                '(%s)' % (who, path, e)) from None
-        _table = module.tensor_table
+        _table = module
+    return _table
+
+
+def _tensor_table(tensors, who):
+    """Addresses, element counts and type codes of contiguous CUDA tensors, as bytes that C reads
+    in place, and their device's index."""
     try:
-        ptrs, numel, codes, device = _table(tensors)
+        ptrs, numel, codes, device = _helper(who).tensor_table(tensors)
     except ValueError as e:
         raise ValueError('%s: %s' % (who, e)) from None
     return ptrs, numel, codes, device if device >= 0 else torch.cuda.current_device()
@@ -707,9 +715,10 @@ def clip_grad_norm(grads, max_norm, *, scale=1.0, eps=1e-6, out=None, sumsq=None
     who = 'grad_clip'
     grads = list(grads)
     ptrs, numel, codes, device = _tensor_table(grads, who)
-    optrs, onumel, ocodes = ptrs, numel, codes
+    optrs, onumel, ocodes, written = ptrs, numel, codes, grads
     if out is not None:
-        optrs, onumel, ocodes, odevice = _tensor_table(list(out), who)
+        written = list(out)
+        optrs, onumel, ocodes, odevice = _tensor_table(written, who)
         if onumel != numel or odevice != device:
             raise ValueError(
                 'grad_clip: out must hold a tensor of the same size and device for each gradient')
@@ -720,4 +729,5 @@ def clip_grad_norm(grads, max_norm, *, scale=1.0, eps=1e-6, out=None, sumsq=None
     _check(lib().cflk_grad_clip(_stream(), len(grads), ptrs, optrs, numel, codes, ocodes,
                                 _ptr(sumsq), float(max_norm), float(eps), float(scale),
                                 _ptr(norm), _ptr(ws), nb), who)
+    _helper(who).mark_written(written)
     return norm

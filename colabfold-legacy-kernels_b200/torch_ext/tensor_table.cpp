@@ -7,6 +7,11 @@
 // the first three bytes objects of int64, int64 and int32 (0 float16, 1 bfloat16, 2 float32), the
 // last the CUDA device's index, or -1 for no tensors. ValueError for anything that is not a
 // contiguous tensor of those types on one CUDA device.
+//
+//   mark_written(sequence) -> None
+//
+// counts an in-place change of each tensor, as torch's own operators do, so that autograd refuses a
+// backward pass over a saved tensor that has since been written.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -86,9 +91,34 @@ PyObject* tensor_table(PyObject*, PyObject* arg) {
     return out;
 }
 
+PyObject* mark_written(PyObject*, PyObject* arg) {
+    PyObject* seq = PySequence_Fast(arg, "a sequence of tensors is wanted");
+    if (seq == nullptr) {
+        return nullptr;
+    }
+    PyObject* out = Py_None;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+    try {
+        for (Py_ssize_t i = 0; out != nullptr && i < n; ++i) {
+            PyObject* item = PySequence_Fast_GET_ITEM(seq, i);
+            if (!THPVariable_Check(item)) {
+                out = refuse("gradients must be tensors");
+            } else if (const at::Tensor& t = THPVariable_Unpack(item); !t.is_inference()) {
+                t.unsafeGetTensorImpl()->bump_version();  // (inference tensors have none)
+            }
+        }
+    } catch (const std::exception& e) {
+        out = refuse(e.what());
+    }
+    Py_DECREF(seq);
+    Py_XINCREF(out);
+    return out;
+}
+
 PyMethodDef methods[] = {
     {"tensor_table", tensor_table, METH_O,
      "Addresses, element counts, type codes and device of a list of tensors."},
+    {"mark_written", mark_written, METH_O, "Count an in-place change of each tensor of a list."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_cflk_table", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

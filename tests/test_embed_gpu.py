@@ -204,3 +204,10 @@ def test_channels_near_2_to_31(C, cuda_device):
     assert int(torch.count_nonzero(got[0])) == 0 and torch.equal(got[1], table[0].float())
     del got, table
     torch.cuda.empty_cache()
+
+
+def test_embed_into_a_tensor_counts_as_a_change_of_it(cuda_device):
+    out = torch.zeros(4, 8, device=cuda_device)
+    v = out._version
+    b200().embed(torch.zeros(4, dtype=torch.int32, device=cuda_device), out[:1].clone(), out=out)
+    assert out._version > v

@@ -167,3 +167,24 @@ def test_sum_of_squares_of_few_elements(cuda_device):
                 t = torch.tensor(np.asarray(a, np.float32), device=cuda_device).to(TD[kind])
                 want = float((a.astype(np.float64) ** 2).sum())
                 assert abs(m.grad_sumsq([t]).item() - want) <= (3 * 2.0 ** -24 + 2.0 ** -50) * want
+
+
+def test_autograd_sees_what_was_written(cuda_device):
+    """Tensors that a call writes count as changed in place; those it only reads do not."""
+    m = b200()
+    p = torch.randn(64, device=cuda_device, requires_grad=True)
+    y = p * 2
+    z = (y * y).sum()  # y is saved
+    m.grad_sumsq([y.detach()])
+    wide = torch.empty(64, device=cuda_device)
+    v, o = y._version, wide._version
+    m.clip_grad_norm([y.detach()], .5, out=[wide])
+    assert y._version == v and wide._version > o
+    m.clip_grad_norm([y.detach()], .5)
+    assert y._version > v
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        z.backward()
+    with torch.inference_mode():
+        t = torch.ones(8, device=cuda_device)
+    m.clip_grad_norm([t], .5)  # has no version
+    assert abs(t.norm().item() - .5) < 1e-5

@@ -173,3 +173,22 @@ def test_gradients_refuse_more_elements_than_their_workspace_counts_launches_for
         p, m, t = arrays((256,) * n, (one,) * n, (2,) * n)
         rc, msg = call('cflk_grad_sumsq', Z, I64(n), p, m, t, P, P, ctypes.c_size_t(1 << 20))
         assert rc == 1 and msg.startswith('grad_norm: '), (rc, msg)
+
+
+def test_helper_counts_writes():
+    """What marks the tensors that a call wrote as changed, on the CPU."""
+    import torch
+
+    from colabfold_legacy_kernels import b200
+    mark = b200._helper('grad_clip').mark_written
+    a, b = torch.zeros(3), torch.zeros(0)
+    with torch.inference_mode():
+        c = torch.zeros(2)  # has no version
+    before = a._version, b._version
+    mark([a, b, c, a[1:]])  # a view shares its base's
+    assert (a._version, b._version) == (before[0] + 2, before[1] + 1)
+    mark([])
+    with pytest.raises(ValueError, match='tensors'):
+        mark([a, 3])
+    with pytest.raises(TypeError):
+        mark(7)
