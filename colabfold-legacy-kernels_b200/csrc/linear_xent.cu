@@ -943,8 +943,9 @@ bool make_plan(int64_t T, int64_t V, int64_t C, bool bwd, Plan& p) {
     // Both sides, in us (head kernels / the tiles below), forward and backward: T 589824, V 64,
     // C 128, nine tenths labelled 37 / 172 and 83 / 615; T 262144, V 23, C 256, 15 % labelled
     // 17 / 30 and 51 / 142, all 30 / 108 and 83 / 387; T 100000, V 128, C 128 16 / 46 and 37 / 151;
-    // T 1000, V 64, C 128 8.1 / 12.7 and 14 / 38; T 50000, V 100, C 200 14 / 32 and 110 / 108 (the
-    // widest that fit, and odd channels, break even backward).
+    // T 1000, V 64, C 128 8.1 / 12.7 and 14 / 38; T 50000, V 100, C 200 forward 14 / 32. Backward
+    // that width (V above 64 with C above 128) does not fit the heads' shared memory and takes the
+    // tiles: 95 to 110.
     p.head = xent_head_fits(V, C, bwd);
     if (p.head) {
         p.bytes = xent_head_workspace(T, V, C, bwd);
