@@ -371,6 +371,13 @@ int check_tensors(const char* who, int64_t n, const void* const* src, void* cons
             if (dst[i] == nullptr || reinterpret_cast<uintptr_t>(dst[i]) % ed != 0) {
                 return bad("a tensor's pointer is null or not aligned to its type");
             }
+            // in place each element is read and written by one thread; otherwise nothing orders them
+            const uintptr_t a = reinterpret_cast<uintptr_t>(src[i]);
+            const uintptr_t b = reinterpret_cast<uintptr_t>(dst[i]);
+            const size_t m = (size_t)numel[i];
+            if ((a != b || es != ed) && a < b + m * ed && b < a + m * es) {
+                return bad("an output overlaps its gradient without being it");
+            }
         }
     }
     return kOk;

@@ -332,10 +332,10 @@ CFLK_API int cflk_grad_sumsq(void* stream, int64_t n, const void* const* grads,
 
 /* norm = scale * sqrt(sum of squares) and outs = grads * scale * min(1, max_norm / (norm + eps)),
  * rounded once. scale > 0 takes a loss scale out. outs[i] may be grads[i] (then nothing is moved
- * when the factor is 1); out_dtypes[i] is dtypes[i], or CFLK_F32 for a buffer of its own. sumsq NULL: the
- * sum is taken of these tensors; otherwise it is read from the device (the sum of the shards of
- * several ranks). norm (device, float32) or NULL. A norm that is not finite gives what the
- * formula gives: zeros and NaN for an infinite one, NaN for NaN. */
+ * when the factor is 1) and overlaps no tensor otherwise; out_dtypes[i] is dtypes[i], or CFLK_F32 for
+ * a buffer of its own. sumsq NULL: the sum is taken of these tensors; otherwise it is read from the
+ * device (the sum of the shards of several ranks). norm (device, float32) or NULL. A norm that is
+ * not finite gives what the formula gives: zeros and NaN for an infinite one, NaN for NaN. */
 CFLK_API int cflk_grad_clip(void* stream, int64_t n, const void* const* grads, void* const* outs,
                             const int64_t* numel, const int* dtypes, const int* out_dtypes,
                             const double* sumsq, float max_norm, float eps, float scale,

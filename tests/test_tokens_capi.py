@@ -168,11 +168,12 @@ def test_gradients_refuse_more_elements_than_their_workspace_counts_launches_for
     """A launch takes 900 tensors and below 2^31 chunks of 2^14 elements; a launch more would write past
     the workspace."""
     for n, one in ((4, 1 << 43), (900, 40 << 30)):
-        rc, msg = clip((256,) * n, (one,) * n, (2,) * n, (256,) * n, (2,) * n)
-        assert rc == 1 and msg.startswith('grad_clip: '), (rc, msg)
+        # (without a workspace, so that no call can get to a launch)
+        rc, msg = clip((256,) * n, (one,) * n, (2,) * n, (256,) * n, (2,) * n, ws=Z)
+        assert rc == 1 and msg.startswith('grad_clip: ') and '2^45' in msg, (rc, msg)
         p, m, t = arrays((256,) * n, (one,) * n, (2,) * n)
-        rc, msg = call('cflk_grad_sumsq', Z, I64(n), p, m, t, P, P, ctypes.c_size_t(1 << 20))
-        assert rc == 1 and msg.startswith('grad_norm: '), (rc, msg)
+        rc, msg = call('cflk_grad_sumsq', Z, I64(n), p, m, t, P, Z, ctypes.c_size_t(1 << 20))
+        assert rc == 1 and msg.startswith('grad_norm: ') and '2^45' in msg, (rc, msg)
 
 
 def test_helper_counts_writes():
@@ -192,3 +193,20 @@ def test_helper_counts_writes():
         mark([a, 3])
     with pytest.raises(TypeError):
         mark(7)
+
+
+@pytest.mark.parametrize('bad', [dict(types=(1, 1), otypes=(2, 1)),  # widened onto itself
+                                 dict(outs=(260, 512)), dict(ptrs=(260, 512), outs=(256, 512)),
+                                 dict(ptrs=(256, 512), numel=(3, 4), outs=(256, 508))])
+def test_clip_refuses_an_output_that_overlaps_its_gradient(bad):
+    # (without a workspace, so that no call can get to a launch)
+    rc, msg = clip(**bad, ws=Z)
+    assert rc == 1 and 'overlaps' in msg
+
+
+@pytest.mark.parametrize('good', [dict(), dict(outs=(268, 528)), dict(ptrs=(268, 528)),
+                                  dict(types=(1, 1), otypes=(2, 1), outs=(264, 520)),
+                                  dict(types=(1, 1), otypes=(2, 1), ptrs=(268, 528))])
+def test_clip_takes_an_output_in_place_or_beside_its_gradient(good):
+    rc, msg = clip(**good, ws=Z)
+    assert rc == 1 and 'workspace' in msg
