@@ -318,8 +318,8 @@ CFLK_API int cflk_linear_xent_bwd(void* stream, int dtype, int labels_64, const 
 
 /* Gradients as n tensors: host arrays of n device pointers, element counts and types (CFLK_F16,
  * CFLK_BF16 or CFLK_F32), read during the call only; a tensor may have no elements, and any
- * alignment its type allows (below 2^44 elements a tensor, 2^45 together). workspace: at least cflk_grad_workspace_size(n) bytes, 8-byte
- * aligned; its contents do not matter.
+ * alignment its type allows (below 2^44 elements a tensor, 2^45 together). workspace: at least
+ * cflk_grad_workspace_size(n) bytes, 8-byte aligned; its contents do not matter.
  *
  * cflk_grad_sumsq: *sumsq (device, float64) = the sum of the squares of all elements. Those of an
  * aligned 16-byte vector (8 or 4 elements) are added in float32, within 3 2^-24 relative, or in
